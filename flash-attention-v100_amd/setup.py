@@ -36,7 +36,7 @@ KERNEL_LIB = os.path.join(LIB_DIR, "libfused_mha.so")
 EXT_LIB = os.path.join(HERE, "flash_attn_v100_cuda.so")
 ROCM_HOME = os.environ.get("ROCM_HOME", "/opt/rocm")
 KERNEL_SOURCES = [os.path.join(CSRC, "fused_mha_kernel.hip"), os.path.join(CSRC, "block_map.h"),
-                  os.path.join(CSRC, "fmha_internal.h"),
+                  os.path.join(CSRC, "fmha_tiles.h"), os.path.join(CSRC, "fmha_internal.h"),
                   os.path.join(INCLUDE, "fused_mha.h")]
 EXT_SOURCES = [os.path.join(CSRC, "fused_mha_api.cpp"), os.path.join(CSRC, "fmha_internal.h"), os.path.join(INCLUDE, "fused_mha.h")]
 
