@@ -15,21 +15,17 @@
 //     with wrong strides;
 //   * the arch gate asks for gfx950 instead of sm_70 (:21-23).
 #include <torch/extension.h>
-#include <ATen/hip/EmptyTensor.h>
-#include <c10/core/DeviceGuard.h>
 #include <c10/hip/HIPCachingAllocator.h>
-#include <c10/hip/HIPFunctions.h>
 #include <c10/hip/HIPGraphsC10Utils.h>
 #include <c10/hip/HIPStream.h>
 #include <hip/hip_runtime_api.h>
 #include <torch/csrc/jit/frontend/tracer.h>
 
 #include <algorithm>
-#include <atomic>
 #include <cmath>
-#include <cstring>
 #include <vector>
 
+#include "api_common.h"
 #include "fused_mha.h"
 #include "fmha_internal.h"
 
@@ -39,24 +35,12 @@
 
 namespace {
 
-void check_arch(int device) {
-  // The property query copies a structure of more than a kilobyte; the answer never changes.
-  static std::atomic<bool> known_gfx950[64];
-  if (device >= 0 && device < 64 && known_gfx950[device].load(std::memory_order_relaxed)) return;
-  hipDeviceProp_t prop;
-  TORCH_CHECK(hipGetDeviceProperties(&prop, device) == hipSuccess, "hipGetDeviceProperties failed");
-  TORCH_CHECK(std::strncmp(prop.gcnArchName, "gfx950", 6) == 0, "This repo only supports gfx950 (MI355X) GPUs, got ",
-              prop.gcnArchName);
-  if (device >= 0 && device < 64) known_gfx950[device].store(true, std::memory_order_relaxed);
-}
+using api::check_arch;
+using api::gpu_empty;
+using api::OnDeviceOf;
 
 void check_rc(int rc, const char* what) {
   TORCH_CHECK(rc == FUSED_MHA_OK, what, " failed: ", fused_mha_error_string(rc));
-}
-
-// torch.empty without the dispatcher, which costs more than the allocation itself.
-at::Tensor gpu_empty(at::IntArrayRef size, at::ScalarType dtype, const at::Tensor& like) {
-  return at::Tensor(at::detail::empty_cuda(size, dtype, like.device(), std::nullopt));
 }
 
 at::Tensor dense(const at::Tensor& x) { return x.is_contiguous() ? x : x.contiguous(); }
@@ -78,14 +62,6 @@ struct Operand {
     copy = x.contiguous();
     ptr = copy.data_ptr();
     st = {copy.stride(0), copy.stride(1), copy.stride(2)};
-  }
-};
-
-// Makes the device of a tensor the current one, which it nearly always is: asking is cheaper than setting it and back.
-struct OnDeviceOf {
-  c10::OptionalDeviceGuard guard;
-  explicit OnDeviceOf(const at::Tensor& x) {
-    if (c10::hip::current_device() != x.get_device()) guard.reset_device(x.device());
   }
 };
 
