@@ -41,7 +41,22 @@ struct PagedArgs {
   int causal, zero_rest;
   int target, least;  // parts aimed at and their least tiles; target 0: an item is a part
   int slots;          // parts there is room for: enough unless entries of ends go back
+  int k_shift, v_shift;  // offsets of 16 positions in the cache are multiples of 2^shift bytes, fewer than 2^32
 };
+
+// The kernel's arguments as they lie in memory, asked for where they are needed again: kept in registers across a main loop they
+// are spilled.
+__device__ __forceinline__ PagedArgs args_again() {
+  typedef __attribute__((address_space(4))) const unsigned Word;
+  Word* from = (Word*)__builtin_amdgcn_kernarg_segment_ptr();
+  asm volatile("" : "+s"(from));
+  struct Words {
+    unsigned w[sizeof(PagedArgs) / 4];
+  } words;
+#pragma unroll
+  for (unsigned i = 0; i < sizeof(PagedArgs) / 4; ++i) words.w[i] = from[i];
+  return __builtin_bit_cast(PagedArgs, words);
+}
 
 struct Sequence {
   int first, n;  // its tokens
@@ -79,6 +94,13 @@ __device__ __forceinline__ int sequence_of(const int* ends, int batch, int t, in
   return min(lo, batch - 1);
 }
 
+// The same address in all lanes, as the copies want it.
+__device__ __forceinline__ const half_t* wave_uniform(const char* p) {
+  const unsigned lo = __builtin_amdgcn_readfirstlane((unsigned)(uintptr_t)p);
+  const unsigned hi = __builtin_amdgcn_readfirstlane((unsigned)((uintptr_t)p >> 32));
+  return (const half_t*)(((uintptr_t)hi << 32) | lo);
+}
+
 __device__ __forceinline__ long sum_over_wave(long x) {
 #pragma unroll
   for (int d = 1; d < 64; d *= 2) x += __shfl_xor(x, d);
@@ -93,60 +115,71 @@ __device__ __forceinline__ int scan_over_wave(int x, int lane) {  // with its ow
   return x;
 }
 
+// Which blocks a launch has: FEW rows for sequences that have at most kFewRows of them, kManyRows for the others; or all of one
+// kind, with FEW = 0 or MANY = false.
+constexpr int kFewRows = 32, kManyRows = 128;
+template <int FEW, bool MANY>
+struct Blocks {
+  static constexpr int kMost = MANY ? kManyRows : FEW;  // rows of a slot
+  static __device__ __forceinline__ bool many(int rows) { return MANY && (FEW == 0 || rows > kFewRows); }
+  static __device__ __forceinline__ int rows_of_block(int rows) { return many(rows) ? kManyRows : FEW; }
+  static __device__ __forceinline__ int count(int rows) { return paged_blocks(rows, rows_of_block(rows)); }
+};
+
 // Tiles of a part.
-template <int ROWS>
+template <typename B>
 __device__ __forceinline__ int tiles_of_part(const PagedArgs& a, int lane) {
   if (a.target == 0) return 1 << 30;
   long tiles = 0;
   for (int b = lane; b < a.batch; b += 64) {
     const Sequence s = sequence(a, b);
-    tiles += (long)paged_blocks(s.n * a.group, ROWS) * paged_tiles(s.keys);
+    tiles += (long)B::count(s.n * a.group) * paged_tiles(s.keys);
   }
-  return paged_tiles_of_part(sum_over_wave(tiles) * a.kv_head, a.target, a.least);
+  return __builtin_amdgcn_readfirstlane(paged_tiles_of_part(sum_over_wave(tiles) * a.kv_head, a.target, a.least));
 }
 
-// Part `w` of the launch, or b = -1; with parts of sequences before it counted in `before`.
+// The part of work group w, or b = -1.
 struct Part {
   int b, head, block, p, parts, number;
   Sequence s;
 };
-template <int ROWS>
+template <typename B>
 __device__ __forceinline__ Part part_of(const PagedArgs& a, int w, int lane) {
-  const int per = tiles_of_part<ROWS>(a, lane);
+  const int per = tiles_of_part<B>(a, lane);
   auto parts_of = [&](int b) __attribute__((always_inline)) {  // of one key head
     if (b >= a.batch) return 0;
     const Sequence s = sequence(a, b);
-    return paged_blocks(s.n * a.group, ROWS) * paged_parts(paged_tiles(s.keys), per);
+    return B::count(s.n * a.group) * paged_parts(paged_tiles(s.keys), per);
   };
   Part r;
   r.b = -1;
   int all = 0;
-  for (int b0 = 0; b0 < a.batch; b0 += 64) all += __shfl(scan_over_wave(parts_of(b0 + lane), lane), 63);
+  for (int b0 = 0; b0 < a.batch; b0 += 64) all += __builtin_amdgcn_readlane(scan_over_wave(parts_of(b0 + lane), lane), 63);
   const int number = paged_spread(w, all * a.kv_head);
-  if (number >= all * a.kv_head) return r;
+  if (number >= all * a.kv_head || (a.target && number >= a.slots)) return r;
   int before = 0;
   for (int b0 = 0; b0 < a.batch; b0 += 64) {
     const int mine = parts_of(b0 + lane), upto = before + scan_over_wave(mine, lane);
     const unsigned long long past = __builtin_amdgcn_ballot_w64(upto * a.kv_head > number);
     if (past) {
       const int l = __builtin_ctzll(past);
-      const int b = b0 + l, of_head = __shfl(mine, l), base = (__shfl(upto, l) - of_head) * a.kv_head;
-      r.b = __builtin_amdgcn_readfirstlane(b);
-      r.s = sequence(a, r.b);
-      if (a.target && number >= a.slots) {
-        r.b = -1;
-        return r;
-      }
+      const int of_head = __builtin_amdgcn_readlane(mine, l), base = (__builtin_amdgcn_readlane(upto, l) - of_head) * a.kv_head;
+      r.b = b0 + l;
+      const Sequence s = sequence(a, r.b);
+      r.s.first = __builtin_amdgcn_readfirstlane(s.first);
+      r.s.n = __builtin_amdgcn_readfirstlane(s.n);
+      r.s.keys = __builtin_amdgcn_readfirstlane(s.keys);
+      r.s.past = __builtin_amdgcn_readfirstlane(s.past);
       r.parts = paged_parts(paged_tiles(r.s.keys), per);
       const int local = number - base;
       r.head = __builtin_amdgcn_readfirstlane(local / of_head);
       const int in_head = local - r.head * of_head;
       r.block = __builtin_amdgcn_readfirstlane(in_head / r.parts);
-      r.p = __builtin_amdgcn_readfirstlane(in_head - r.block * r.parts);
+      r.p = in_head - r.block * r.parts;
       r.number = number;
       return r;
     }
-    before = __shfl(upto, 63);
+    before = __builtin_amdgcn_readlane(upto, 63);
   }
   return r;
 }
@@ -200,7 +233,8 @@ __device__ __forceinline__ float over_groups_sum(float x) {
 // wave's own tile of LDS (converted there from 8 bits), scores are formed transposed, S^T[keys][rows], so that the 16-bit
 // probabilities are the second product's operand as they are (Geom16).  At the end the waves' sums are joined in LDS.
 // ---------------------------------------------------------------------------
-constexpr int kFewWaves = 4;
+constexpr int kPagedThreads = 256;
+constexpr int kFewWaves = kPagedThreads / 64;
 constexpr int kUnit = 32;
 template <int D, int CB>
 struct FewGeom {
@@ -212,24 +246,15 @@ struct FewGeom {
 };
 
 template <int D, int CB, bool BF, bool Q8>
-__global__ void __launch_bounds__(kFewWaves * 64, 2) paged_few_kernel(PagedArgs a) {
+__device__ __forceinline__ void few_rows(const PagedArgs& a, const Part& w, char* smem, float2* joined, int slot_rows) {
   using T = SwzTile<D>;
   using G = FewGeom<D, CB>;
   constexpr int kRows = G::kRows, kNC = T::kNC, kKS = D / 32, kDB = D / 16;
   constexpr int kLoads = Q8 ? kNC / 2 : kNC;  // of 16 positions: 64 bytes of each
-  __shared__ __attribute__((aligned(1024))) char smem[kFewWaves * G::kWaveBytes];
-  __shared__ float2 join[kFewWaves][kRows];
+  float2(*const join)[kRows] = reinterpret_cast<float2(*)[kRows]>(joined);
 
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int m = lane & 15, g = lane >> 4;
-  if (a.zero_rest) {
-    const int rest = min(max(a.ends[a.batch - 1], 0), a.tokens);
-    const long from = (long)rest * a.head * D * 2, to = (long)a.tokens * a.head * D * 2;
-    for (long i = from + ((long)blockIdx.x * blockDim.x + threadIdx.x) * 16; i < to; i += (long)gridDim.x * blockDim.x * 16)
-      *reinterpret_cast<u4v*>(a.o + i) = u4v{0, 0, 0, 0};
-  }
-  const Part w = part_of<kRows>(a, blockIdx.x, lane);
-  if (w.b < 0) return;
   const int rows = w.s.n * a.group, row0 = w.block * kRows;
   const int last_token = (min(rows, row0 + kRows) - 1) / a.group;
   const int seen = paged_visible(w.s.keys, w.s.n, last_token, a.causal);
@@ -424,7 +449,7 @@ __global__ void __launch_bounds__(kFewWaves * 64, 2) paged_few_kernel(PagedArgs 
       const float inv = sum == 0.f ? 0.f : 1.f / sum;
       store4<BF>(a.o + (((long)(w.s.first + token) * a.head + head) * D + piece * 4) * 2, x * inv);
     } else {
-      const long at = (long)w.number * kRows + row;
+      const long at = (long)w.number * slot_rows + row;
       *reinterpret_cast<f4v*>(a.part_o + at * D + piece * 4) = x;
       if (piece == 0) a.part_ml[at] = float2{mx, sum};
     }
@@ -432,10 +457,440 @@ __global__ void __launch_bounds__(kFewWaves * 64, 2) paged_few_kernel(PagedArgs 
 }
 
 // ---------------------------------------------------------------------------
+// Attention, blocks of 128 rows.  Work group = 4 waves of 32 rows each, one per SIMD, two work groups to a CU; K and V in tiles of 64
+// keys with two slots of LDS each, 16 rows of a tile copied by each wave from one page.  The steps are those of the 128-query
+// forward for equal lengths: softmax(j) with the MFMAs of accumulate(j - 1) and scores(j + 1) between its vector
+// instructions, the running maximum raised only where a tile's probabilities come out too large.  New tokens stand anywhere
+// against the tiles, so up to two tiles of a wave need a mask; they are done after the main loop.
+// ---------------------------------------------------------------------------
+template <int D>
+struct ManyGeom {
+  static constexpr int kPitch = 64 * 4 + 16;  // of a row of 64 sums in LDS
+  static constexpr int kTileBytes = 4 * SwzTile<D>::kBytes, kStageBytes = kPagedThreads / 64 * kResident * kPitch;
+  static constexpr int kBytes = kTileBytes > kStageBytes ? kTileBytes : kStageBytes;
+};
+constexpr float kNoMaximum = -3.4028234663852886e38f;  // in the place of -inf: a difference of two of them is 0
+
+template <bool BF>
+__device__ __forceinline__ f16v mma32(h8 x, h8 y, f16v z) {
+  if constexpr (BF) return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(b8, x), __builtin_bit_cast(b8, y), z, 0, 0, 0);
+  else return mfma(x, y, z);
+}
+// pack2 at this place in the program: seen through, the optimiser moves conversions past the next branch.
+template <bool BF>
+__device__ __forceinline__ unsigned pack2_here(float x, float y) {
+  unsigned r = pack2<BF>(x, y);
+  asm volatile("" : "+v"(r));
+  return r;
+}
+
+template <int D, bool BF>
+__device__ __forceinline__ void many_rows(const PagedArgs& a, const Part& w, char* smem, int* bad_pages) {
+  using G = TileGeom<D>;
+  using T = SwzTile<D>;
+  constexpr int kDB = G::kDBlocks, kIPW = T::kNC;  // copies of a wave and tile: 16 rows, 64 bytes of each
+  constexpr int kVOff = 2 * T::kBytes;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  // what depends on the lane is worked out again where it is needed, not kept in registers across the main loop
+  auto lane_now = []() __attribute__((always_inline)) {
+    int t = threadIdx.x;
+    asm volatile("" : "+v"(t));
+    return t & 63;
+  };
+  const int rows = w.s.n * a.group, row0 = w.block * kManyRows, row0w = row0 + wave * kResident;
+  int t0, t1;
+  paged_part(paged_tiles(paged_visible(w.s.keys, w.s.n, (min(rows, row0 + kManyRows) - 1) / a.group, a.causal)), w.parts, w.p, t0, t1);
+  const int nt = t1 - t0;
+  int ntw = 0, nfull = 0;  // tiles that the wave works on, those of them that all its rows see whole
+  if (row0w < rows) {
+    ntw = min(max(paged_tiles(paged_visible(w.s.keys, w.s.n, (min(rows, row0w + kResident) - 1) / a.group, a.causal)) - t0, 0), nt);
+    nfull = min(max(paged_visible(w.s.keys, w.s.n, row0w / a.group, a.causal) / kPagedTile - t0, 0), nt);
+  }
+  const int jm = min(nfull, ntw - 1);  // steps of the main loop, with the first
+
+  // Offsets in the cache of this wave's 16 rows of 64 tiles, lane l those of tile from + l; in the lane's registers.
+  const char* const k_head = a.k + (long)w.head * a.ks.head;
+  const char* const v_head = a.v + (long)w.head * a.vs.head;
+  const int last_stretch = (w.s.keys - 1) >> 4;
+  const int k_shift = a.k_shift, v_shift = a.v_shift;
+  unsigned k_at = 0, v_at = 0;
+  int at_from = 0;
+  bool bad = w.s.past;
+  auto fetch_at = [&](int j) __attribute__((always_inline)) {
+    at_from = j;
+    const PagedArgs a = args_again();
+    const int lane = lane_now(), stretch = min(4 * (t0 + j + lane) + wave, last_stretch);
+    const int pos = stretch * 16, page_at = pos / a.page_size, slot = pos - page_at * (int)a.page_size;
+    int id = a.table[w.b * a.table_stride + page_at];
+    const bool none = (unsigned)id >= (unsigned)a.pages;
+    bad |= __builtin_amdgcn_ballot_w64(none && j + lane < nt) != 0;
+    if (none) id = 0;
+    k_at = (unsigned)((id * a.ks.page + (long)slot * a.ks.slot) >> a.k_shift);
+    v_at = (unsigned)((id * a.vs.page + (long)slot * a.vs.slot) >> a.v_shift);
+    asm volatile("" : "+v"(k_at), "+v"(v_at));
+  };
+  constexpr int kBack = 960 * (kIPW - 1);  // see copy16_blocks
+  int k_goff, v_goff;
+  {
+    const int lane = lane_now(), r16 = lane >> 2, col = ((lane & 3) ^ swz(r16 >> 2)) * 16;
+    k_goff = r16 * a.ks.slot + col + kBack;
+    v_goff = r16 * a.vs.slot + col + kBack;
+    asm volatile("" : "+v"(k_goff), "+v"(v_goff));
+  }
+  const unsigned lds0 = (unsigned)(uintptr_t)(__attribute__((address_space(3))) char*)smem;
+  const unsigned lds_w = lds0 + wave * (kIPW * 1024);
+  // K(j) and V(j - 2) are asked for in the same step: V comes out of the same registers two tiles later, before they are fetched anew
+  auto past_end = [&](int j, int off, bool value) __attribute__((always_inline)) {  // rows behind the last key: that one
+    const PagedArgs a = args_again();
+    const int stride = value ? a.vs.slot : a.ks.slot;
+    const int lane = lane_now(), stretch = min(4 * (t0 + j) + wave, last_stretch);
+    const int r16 = lane >> 2;
+    return off - max(r16 - (w.s.keys - 1 - stretch * 16), 0) * stride;
+  };
+  const int j_end = (w.s.keys - 1) / kPagedTile - t0;  // the tile with the last key
+  auto copy_k = [&](int j, int slot) __attribute__((always_inline)) {
+    const char* const from = k_head + ((long)(unsigned)__builtin_amdgcn_readlane(k_at, j - at_from) << k_shift) - kBack;
+    int off = k_goff;
+    if (j == j_end) off = past_end(j, off, false);
+    copy16_blocks<kIPW>(wave_uniform(from), off, __builtin_amdgcn_readfirstlane(lds_w + slot * T::kBytes));
+  };
+  auto copy_v = [&](int j, int slot) __attribute__((always_inline)) {
+    const char* const from = v_head + ((long)(unsigned)__builtin_amdgcn_readlane(v_at, j - at_from) << v_shift) - kBack;
+    int off = v_goff;
+    if (j == j_end) off = past_end(j, off, true);
+    copy16_blocks<kIPW>(wave_uniform(from), off, __builtin_amdgcn_readfirstlane(lds_w + kVOff + slot * T::kBytes));
+  };
+
+  // the block's rows of q fill the slots of V, which comes later
+  char* const my_rows = smem + kVOff + wave * (T::kBytes / 2);
+  {
+    const int lane = lane_now(), r16 = lane >> 2, col = ((lane & 3) ^ swz(r16 >> 2)) * 16;
+    const char* const base = a.q + w.b * a.q_batch + (a.ends ? w.s.first : 0) * a.q_seq + (long)w.head * (int)a.group * a.q_head;
+#pragma unroll
+    for (int R = 0; R < 2; ++R) {
+      const int row = min(row0w + 16 * R + r16, rows - 1), token = row / a.group;
+      const char* const from = base + token * a.q_seq + (row - token * (int)a.group) * a.q_head + col;
+#pragma unroll
+      for (int C = 0; C < T::kNC; ++C)
+        *reinterpret_cast<u4v*>(my_rows + T::block_off(R, C) + lane * 16) = *reinterpret_cast<const u4v*>(from + C * 64);
+    }
+  }
+  if (nt > 0) {
+    fetch_at(0);
+    copy_k(0, 0);
+    if (nt > 1) copy_k(1, 1);
+  }
+  h8 qf[G::kKSteps];
+  {
+    const StagedRows<D> staged{my_rows, lane_now()};
+    staged_rows_read();
+#pragma unroll
+    for (int kk = 0; kk < G::kKSteps; ++kk) qf[kk] = staged.wide(kk);
+    staged_rows_read();
+  }
+  if (!(a.c > 0.f)) {  // the maximum of scores times c is c times their maximum only for c > 0
+#pragma unroll
+    for (int kk = 0; kk < G::kKSteps; ++kk) {
+      qf[kk] = a.c < 0.f ? -qf[kk] : h8{};
+      asm volatile("" : "+v"(qf[kk]));
+    }
+  }
+  const float c = a.c == 0.f ? 1.f : fabsf(a.c);
+  int k_off[2], v_off[2];
+  swz_rows_off<D>(lane_now(), k_off);
+  swz_cols_off<D>(lane_now(), v_off);
+  const unsigned ka0 = opaque_lds_address(smem + k_off[0]), ka1 = opaque_lds_address(smem + k_off[1]);
+  const unsigned va0 = opaque_lds_address(smem + v_off[0]), va1 = opaque_lds_address(smem + v_off[1]);
+  auto k_frag = [&](unsigned at, int n) __attribute__((always_inline)) { return swz_rows_at<D>(ka0 + at, ka1 + at, n & 1, n >> 1); };
+  auto v_frag = [&](unsigned at, int n) __attribute__((always_inline)) {
+    return swz_cols_at<D>(va0 + kVOff + at, va1 + kVOff + at, n / kDB, n % kDB);
+  };
+
+  f16v o[kDB], zero;
+#pragma unroll
+  for (int r = 0; r < 16; ++r) zero[r] = 0.f;
+#pragma unroll
+  for (int db = 0; db < kDB; ++db) o[db] = zero;
+  float mc = kNoMaximum, l_run = 0.f;
+  f16v sA[2], sB[2];
+  u4v pf[4];  // probabilities of a tile, pairs of 16 bits in B-operand order
+
+  constexpr int kLead = 3;  // LDS fragments are read this many MFMAs ahead
+  constexpr int kNS = 2 * G::kKSteps, kNP = 4 * kDB;
+  auto scores = [&](unsigned at, f16v (&s)[2]) __attribute__((always_inline)) {
+    h8 frag[kLead];
+#pragma unroll
+    for (int n = 0; n < kLead; ++n) frag[n] = k_frag(at, n);
+    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+    for (int n = 0; n < kNS; ++n) {
+      const int rb = n & 1, kk = n >> 1;
+      s[rb] = mma32<BF>(frag[n % kLead], qf[kk], kk == 0 ? zero : s[rb]);
+      if (n + kLead < kNS) frag[n % kLead] = k_frag(at, n + kLead);
+      __builtin_amdgcn_sched_barrier(0);
+    }
+  };
+  auto exponentials = [&](const f16v (&s)[2]) __attribute__((always_inline)) {
+    float l0 = 0.f, l1 = 0.f;
+#pragma unroll
+    for (int c16 = 0; c16 < 4; ++c16) {
+#pragma unroll
+      for (int e = 0; e < 8; e += 2) {
+        const float p0 = fast_exp2(fmaf(s[c16 >> 1][(c16 & 1) * 8 + e], c, -mc));
+        const float p1 = fast_exp2(fmaf(s[c16 >> 1][(c16 & 1) * 8 + e + 1], c, -mc));
+        pf[c16][e >> 1] = pack2_here<BF>(p0, p1);
+        l0 += p0;
+        l1 += p1;
+      }
+      __builtin_amdgcn_sched_barrier(0);
+    }
+    return l0 + l1;
+  };
+  auto mask = [&](f16v (&s)[2], int j) __attribute__((always_inline)) {
+    const PagedArgs a = args_again();
+    const int lane = lane_now(), token = min(row0w + (lane & 31), rows - 1) / a.group;
+    const int left = paged_visible(w.s.keys, w.s.n, token, a.causal) - (t0 + j) * kPagedTile - 4 * (lane >> 5);
+#pragma unroll
+    for (int rb = 0; rb < 2; ++rb)
+#pragma unroll
+      for (int r = 0; r < 16; ++r)
+        if (acc_row(rb, r, 0) >= left) s[rb][r] = -INFINITY;
+  };
+  auto too_large = [&](float lt) __attribute__((always_inline)) { return __builtin_amdgcn_ballot_w64(!(lt <= 4096.f)) != 0; };
+  // probabilities of a tile with the running maximum brought up to date
+  auto raise_max = [&](const f16v (&s)[2]) __attribute__((always_inline)) {
+    float mx = s[0][0];
+#pragma unroll
+    for (int rb = 0; rb < 2; ++rb)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) mx = fmaxf(mx, s[rb][r]);
+    mx = fmaxf(mx, other_half(mx));
+    const float mc_new = fmaxf(mc, mx * c);
+    const float alpha = fast_exp2(mc - mc_new);
+    mc = mc_new;
+    l_run *= alpha;
+#pragma unroll
+    for (int db = 0; db < kDB; ++db)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) o[db][r] *= alpha;
+    l_run += exponentials(s);
+  };
+  auto accumulate = [&](unsigned at) __attribute__((always_inline)) {
+    h8 frag[kLead];
+#pragma unroll
+    for (int n = 0; n < kLead; ++n) frag[n] = v_frag(at, n);
+    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+    for (int n = 0; n < kNP; ++n) {
+      o[n % kDB] = mma32<BF>(frag[n % kLead], __builtin_bit_cast(h8, pf[n / kDB]), o[n % kDB]);
+      if (n + kLead < kNP) frag[n % kLead] = v_frag(at, n + kLead);
+      __builtin_amdgcn_sched_barrier(0);
+    }
+  };
+  // Step j uses K(j + 1) and V(j - 1), both in slot (j + 1) & 1; K(j + 2) and V(j) are copied into the other one.
+  auto top_wait = [&]() __attribute__((always_inline)) {
+    wait_vm<0>();
+    block_barrier();
+  };
+  auto fetch_for = [&](int j) __attribute__((always_inline)) {  // the registers hold tiles at_from .. at_from + 63
+    if (j + 2 - at_from >= 64 && j < nt) fetch_at(j);
+  };
+  auto top_copy = [&](int j, int slot) __attribute__((always_inline)) {
+    fetch_for(j);
+    if (j + 2 < nt) copy_k(j + 2, slot);
+    if (j < nt) copy_v(j, slot);
+  };
+  auto step = [&](int j, auto slot_tag, const f16v (&s)[2], f16v (&sn)[2]) __attribute__((always_inline)) {
+    constexpr int kSlot = decltype(slot_tag)::value;  // (j + 1) & 1
+    constexpr unsigned at = kSlot * T::kBytes;
+    constexpr int kM = kNS + kNP;
+    h8 frag[kLead];
+    float l0 = 0.f, l1 = 0.f, p0 = 0.f, p1 = 0.f;
+    auto read = [&](int m) __attribute__((always_inline)) {
+      const int ch = m / (2 * kDB), in = m % (2 * kDB);
+      return in < kDB ? v_frag(at, ch * kDB + in) : k_frag(at, ch * kDB + in - kDB);
+    };
+    auto reads = [](int m) { return m >= kM ? 0 : m % (2 * kDB) < kDB ? 2 : 1; };  // LDS reads of a fragment
+    auto start = [&](int x) __attribute__((always_inline)) {
+      const int c16 = x >> 2, e = (x & 3) * 2;
+      p0 = fast_exp2(fmaf(s[c16 >> 1][(c16 & 1) * 8 + e], c, -mc));
+      p1 = fast_exp2(fmaf(s[c16 >> 1][(c16 & 1) * 8 + e + 1], c, -mc));
+    };
+    auto finish = [&](int x) __attribute__((always_inline)) {
+      const int c16 = x >> 2, e = (x & 3) * 2;
+      l0 += p0;
+      l1 += p1;
+      asm volatile("" : "+v"(l0), "+v"(l1));  // sums now, not all at the end
+      pf[c16][e >> 1] = pack2_here<BF>(p0, p1);
+    };
+    top_wait();
+    fetch_for(j);
+#pragma unroll
+    for (int m = 0; m < kLead; ++m) frag[m] = read(m);
+    constexpr int kCopyKAt = D == 128 ? 8 : 0;  // K's copies follow when V's are through
+    copy_v(j, 1 - kSlot);
+    if (kCopyKAt == 0 && j + 2 < nt) copy_k(j + 2, 1 - kSlot);
+    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+    for (int m = 0; m < kM + 2; ++m) {
+      if (kCopyKAt != 0 && m == kCopyKAt && j + 2 < nt) copy_k(j + 2, 1 - kSlot);
+      if (m < kM && m % 2 == 0) {  // one wait for the fragments of this unit and the next
+        if (D == 64) wait_lds_pinned(reads(m + 2));
+        else wait_lds(reads(m + 2));
+      }
+      if (m < kM) {
+        const int ch = m / (2 * kDB), in = m % (2 * kDB);
+        if (in < kDB) {
+          o[in] = mma32<BF>(frag[m % kLead], __builtin_bit_cast(h8, pf[ch]), o[in]);
+        } else {
+          const int n = ch * kDB + in - kDB, rb = n & 1, kk = n >> 1;
+          sn[rb] = mma32<BF>(frag[m % kLead], qf[kk], kk == 0 ? zero : sn[rb]);
+        }
+        if (m + kLead < kM) frag[m % kLead] = read(m + kLead);
+      }
+      if (D == 64) {
+        if (m >= 1 && m - 1 < 16) finish(m - 1);
+        if (m < 16) start(m);
+      } else {
+        if (m & 1) {
+          if (m >= 3 && m < 35) finish((m - 3) / 2);
+        } else if (m >= 2 && m < 34) {
+          start((m - 2) / 2);
+        }
+      }
+      __builtin_amdgcn_sched_barrier(0);
+    }
+    return l0 + l1;
+  };
+
+  if (nt > 1) wait_vm<kIPW>();  // the second tile of K may still be on its way
+  else wait_vm<0>();
+  block_barrier();
+  if (ntw > 0) scores(0, sA);
+  int j = 0;
+  if (jm > 0) {
+    top_wait();
+    top_copy(0, 0);
+    scores(T::kBytes, sB);
+    raise_max(sA);
+    ++j;
+#pragma unroll
+    for (int rb = 0; rb < 2; ++rb) sA[rb] = sB[rb];
+    // two tiles per round, the scores alternating between two sets of registers
+    bool odd_done = false;
+    for (;;) {
+      int why;
+      for (;;) {
+        if (!odd_done) {
+          if (j >= jm) { why = 0; break; }
+          const float lt = step(j, IntTag<0>{}, sA, sB);
+          if (too_large(lt)) { why = 1; break; }
+          l_run += lt;
+          ++j;
+        }
+        odd_done = false;
+        if (j >= jm) { why = 2; break; }
+        const float lt = step(j, IntTag<1>{}, sB, sA);
+        if (too_large(lt)) { why = 3; break; }
+        l_run += lt;
+        ++j;
+      }
+      if (why == 0) break;
+      if (why == 2) {
+#pragma unroll
+        for (int rb = 0; rb < 2; ++rb) sA[rb] = sB[rb];
+        break;
+      }
+      if (why == 1) raise_max(sA);
+      else raise_max(sB);
+      ++j;
+      odd_done = why == 1;
+    }
+  }
+  // the wave's last tiles (up to two with a mask) and the accumulation after them; it goes on copying for the others
+  for (; j <= nt; ++j) {
+    const unsigned at = ((j + 1) & 1) * T::kBytes;
+    top_wait();
+    top_copy(j, j & 1);
+    if (j > 0 && j <= ntw) accumulate(at);
+    if (j < ntw) {
+      mask(sA, j);
+      raise_max(sA);
+      if (j + 1 < ntw) scores(at, sA);
+    }
+  }
+
+  bad_pages[wave] = bad;  // each wave has looked at a quarter of the pages
+  block_barrier();        // every wave is done with the rings: they become the staging tiles
+  const PagedArgs z = args_again();
+  const int lane = lane_now();
+  float l_tot = l_run + other_half(l_run);
+  if (bad_pages[0] | bad_pages[1] | bad_pages[2] | bad_pages[3]) l_tot = NAN;
+  const float f = w.parts > 1 ? 1.f : l_tot == 0.f ? 0.f : 1.f / l_tot;
+  char* const stage = smem + wave * (kResident * ManyGeom<D>::kPitch);
+  const long slot0 = (long)w.number * kManyRows + wave * kResident;
+  if (w.parts > 1 && lane < kResident && row0w + lane < rows) z.part_ml[slot0 + lane] = float2{mc, l_tot};
+#pragma unroll
+  for (int half = 0; half < D / 64; ++half) {
+#pragma unroll
+    for (int db = 0; db < 2; ++db)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        f4v x;
+#pragma unroll
+        for (int r = 0; r < 4; ++r) x[r] = o[2 * half + db][4 * e + r] * f;
+        *reinterpret_cast<f4v*>(stage + (lane & 31) * ManyGeom<D>::kPitch + (db * 32 + 8 * e + 4 * (lane >> 5)) * 4) = x;
+      }
+    __builtin_amdgcn_s_waitcnt(0xC07F);  // lgkmcnt(0): the wave's own writes have landed
+    asm volatile("" ::: "memory");
+#pragma unroll
+    for (int pass = 0; pass < kResident / 4; ++pass) {
+      const int r = 4 * pass + (lane >> 4), row = row0w + r, piece = lane & 15;
+      const f4v x = *reinterpret_cast<const f4v*>(stage + r * ManyGeom<D>::kPitch + piece * 16);
+      if (row < rows) {
+        if (w.parts > 1) {
+          *reinterpret_cast<f4v*>(z.part_o + (slot0 + r) * D + half * 64 + piece * 4) = x;
+        } else {
+          const int token = row / z.group, head = w.head * (int)z.group + row - token * (int)z.group;
+          store4<BF>(z.o + (((long)(w.s.first + token) * z.head + head) * D + half * 64 + piece * 4) * 2, x);
+        }
+      }
+    }
+    __builtin_amdgcn_s_waitcnt(0xC07F);
+    asm volatile("" ::: "memory");
+  }
+}
+
+// ---------------------------------------------------------------------------
+// A work group's part, by whichever of the two ways its sequence goes.
+// ---------------------------------------------------------------------------
+template <int D, int FEW, bool MANY, bool BF, bool Q8>
+__global__ void __launch_bounds__(kPagedThreads, 2) paged_forward_kernel(PagedArgs a) {
+  using B = Blocks<FEW, MANY>;
+  constexpr int kFewBytes = FEW ? kFewWaves * FewGeom<D, FEW ? FEW / 16 : 1>::kWaveBytes : 0, kManyBytes = MANY ? ManyGeom<D>::kBytes : 0;
+  __shared__ __attribute__((aligned(1024))) char smem[kFewBytes > kManyBytes ? kFewBytes : kManyBytes];
+  __shared__ float2 joined[FEW ? kFewWaves * FEW : 1];
+  __shared__ int bad_pages[kFewWaves];
+  if (a.zero_rest) {
+    const int rest = min(max(a.ends[a.batch - 1], 0), a.tokens);
+    const long from = (long)rest * a.head * D * 2, to = (long)a.tokens * a.head * D * 2;
+    for (long i = from + ((long)blockIdx.x * blockDim.x + threadIdx.x) * 16; i < to; i += (long)gridDim.x * blockDim.x * 16)
+      *reinterpret_cast<u4v*>(a.o + i) = u4v{0, 0, 0, 0};
+  }
+  const Part w = part_of<B>(a, blockIdx.x, threadIdx.x & 63);
+  if (w.b < 0) return;
+  if constexpr (MANY) {
+    if (B::many(w.s.n * a.group)) return many_rows<D, BF>(a, w, smem, bad_pages);
+  }
+  if constexpr (FEW != 0) few_rows<D, FEW / 16, BF, Q8>(a, w, smem, joined, B::kMost);
+}
+
+// ---------------------------------------------------------------------------
 // Rows whose keys went to several parts.  A work group has one row of the output: D / 4 threads to a part's row.
 // ---------------------------------------------------------------------------
-template <int D, int ROWS, bool BF>
+template <int D, typename B, bool BF>
 __global__ void __launch_bounds__(256) paged_join_kernel(PagedArgs a) {
+  constexpr int ROWS = B::kMost;
   constexpr int kPieces = D / 4, kSlices = 256 / kPieces;
   __shared__ f4v sums[kSlices][kPieces];
   const int lane = threadIdx.x & 63;
@@ -444,19 +899,20 @@ __global__ void __launch_bounds__(256) paged_join_kernel(PagedArgs a) {
   const Sequence s = sequence(a, b);
   const int i = token - s.first;
   if (i < 0 || i >= s.n) return;
-  const int per = tiles_of_part<ROWS>(a, lane);
+  const int per = tiles_of_part<B>(a, lane);
   const int parts = paged_parts(paged_tiles(s.keys), per);
   if (parts == 1) return;
   int before = 0;
   for (int b0 = lane; b0 < b; b0 += 64) {
     const Sequence t = sequence(a, b0);
-    before += paged_blocks(t.n * a.group, ROWS) * paged_parts(paged_tiles(t.keys), per);
+    before += B::count(t.n * a.group) * paged_parts(paged_tiles(t.keys), per);
   }
   before = (int)sum_over_wave(before);
-  const int kvh = head / a.group, row = i * a.group + head - kvh * a.group, block = row / ROWS;
-  const long first = (long)before * a.kv_head + ((long)kvh * paged_blocks(s.n * a.group, ROWS) + block) * parts;
+  const int kvh = head / a.group, row = i * a.group + head - kvh * a.group;
+  const int rows_of_block = B::rows_of_block(s.n * a.group), block = row / rows_of_block;
+  const long first = (long)before * a.kv_head + ((long)kvh * B::count(s.n * a.group) + block) * parts;
   if (first + parts > a.slots) return;
-  const long at = first * ROWS + row % ROWS;
+  const long at = first * ROWS + row % rows_of_block;
   float mx = -INFINITY;
   for (int p = lane; p < parts; p += 64) mx = fmaxf(mx, a.part_ml[at + (long)p * ROWS].x);
 #pragma unroll
@@ -667,30 +1123,41 @@ long all_tokens(const paged_mha_batch* b) { return b->cu_seqlens ? b->tokens : (
 constexpr int kTarget = 512, kLeast = 4;
 
 struct Launch {
-  int rows_of_block;
+  int few;    // rows of a block of few, 0: there is none
+  bool many;  // whether there are blocks of kManyRows
   long items;  // at most
   int target;
+  int slot_rows() const { return many ? kManyRows : few; }
   long slots() const { return target ? items + target : 0; }
   long grid() const { return (items + target + 7) / 8 * 8; }
 };
+// The bits below which all offsets of 16 positions are 0, and whether the bits above fit 32.
+bool fits(const paged_mha_cache* c, const paged_mha_strides& s, int bytes, int& shift) {
+  const unsigned long long page = s.page * bytes, slot = s.slot * bytes * 16, any = page | slot;
+  shift = any ? std::min(__builtin_ctzll(any), 31) : 4;
+  return ((page * (c->pages - 1) + slot * (c->page_size / 16)) >> shift) < (1ull << 32);
+}
 Launch plan(const paged_mha_cache* c, const paged_mha_batch* b, int head, int max_new) {
   const long group = head / c->kv_head;
-  const long most = b->cu_seqlens ? (max_new > 0 ? std::min<long>(max_new, b->tokens) : b->tokens) : b->tokens;
+  const long most = (b->cu_seqlens && max_new > 0 ? std::min(max_new, b->tokens) : b->tokens) * group;
+  int shift;
   Launch p;
-  p.rows_of_block = most * group <= 16 ? 16 : 32;
-  const long blocks = b->cu_seqlens ? b->tokens * group / p.rows_of_block + b->batch : b->batch * ((b->tokens * group + p.rows_of_block - 1) / p.rows_of_block);
+  p.many = most > kFewRows && c->cache_type == c->type && fits(c, c->key_strides, 2, shift) && fits(c, c->value_strides, 2, shift);
+  p.few = most <= 16 ? 16 : !p.many || b->cu_seqlens ? kFewRows : 0;
+  const int least_rows = p.few ? p.few : kManyRows;
+  const long blocks = b->cu_seqlens ? b->tokens * group / least_rows + b->batch : b->batch * ((b->tokens * group + least_rows - 1) / least_rows);
   p.items = blocks * c->kv_head;
   p.target = (long)b->table_width * c->page_size > kLeast * kPagedTile ? kTarget : 0;
   return p;
 }
-size_t workspace_bytes_of(const Launch& p, int d) { return (size_t)p.slots() * p.rows_of_block * (d * 4 + 8); }
+size_t workspace_bytes_of(const Launch& p, int d) { return (size_t)p.slots() * p.slot_rows() * (d * 4 + 8); }
 
-template <int D, int CB, bool BF, bool Q8>
-int launch_few(const Launch& p, const PagedArgs& a, hipStream_t stream) {
-  if (launch(paged_few_kernel<D, CB, BF, Q8>, dim3(p.grid()), kFewWaves * 64, stream, a) != hipSuccess) return FUSED_MHA_ERR_LAUNCH;
+template <int D, int FEW, bool MANY, bool BF, bool Q8>
+int launch_forward(const Launch& p, const PagedArgs& a, hipStream_t stream) {
+  if (launch(paged_forward_kernel<D, FEW, MANY, BF, Q8>, dim3(p.grid()), kPagedThreads, stream, a) != hipSuccess) return FUSED_MHA_ERR_LAUNCH;
   if (!p.target) return FUSED_MHA_OK;
   const long rows = (long)a.tokens * a.head;
-  return launch(paged_join_kernel<D, 16 * CB, BF>, dim3(rows), 256, stream, a) == hipSuccess ? FUSED_MHA_OK : FUSED_MHA_ERR_LAUNCH;
+  return launch(paged_join_kernel<D, Blocks<FEW, MANY>, BF>, dim3(rows), 256, stream, a) == hipSuccess ? FUSED_MHA_OK : FUSED_MHA_ERR_LAUNCH;
 }
 
 // f(D, BF, Q8) with the values of a cache as constants.
@@ -790,7 +1257,7 @@ int paged_mha_forward(const paged_mha_cache* c, const paged_mha_batch* b, const 
   a.k_scale = (const unsigned char*)c->key_scale, a.v_scale = (const unsigned char*)c->value_scale;
   a.table = b->page_table, a.keys = b->cache_seqlens, a.ends = b->cu_seqlens ? b->cu_seqlens + 1 : nullptr;
   a.part_o = (float*)workspace;
-  a.part_ml = (float2*)((char*)workspace + (size_t)p.slots() * p.rows_of_block * c->d * 4);
+  a.part_ml = (float2*)((char*)workspace + (size_t)p.slots() * p.slot_rows() * c->d * 4);
   a.ks = in_bytes(c->key_strides, bytes), a.vs = in_bytes(c->value_strides, bytes);
   a.kss = in_bytes(c->key_scale_strides, 1), a.vss = in_bytes(c->value_scale_strides, 1);
   a.q_batch = a.ends ? 0 : q_st->batch * 2, a.q_seq = q_st->seq * 2, a.q_head = q_st->head * 2;
@@ -801,10 +1268,15 @@ int paged_mha_forward(const paged_mha_cache* c, const paged_mha_batch* b, const 
   a.c = scale * kLog2e;
   a.causal = causal != 0, a.zero_rest = zero_rest != 0 && a.ends;
   a.target = p.target, a.least = kLeast, a.slots = (int)p.slots();
+  if (p.many) fits(c, c->key_strides, 2, a.k_shift), fits(c, c->value_strides, 2, a.v_shift);
   return with_types(c, [&](auto d, auto bf, auto q8) {
     constexpr int D = decltype(d)::value;
     constexpr bool BF = decltype(bf)::value != 0, Q8 = decltype(q8)::value != 0;
-    return p.rows_of_block == 16 ? launch_few<D, 1, BF, Q8>(p, a, (hipStream_t)stream) : launch_few<D, 2, BF, Q8>(p, a, (hipStream_t)stream);
+    const hipStream_t st = (hipStream_t)stream;
+    if constexpr (!Q8) {
+      if (p.many) return p.few ? launch_forward<D, kFewRows, true, BF, Q8>(p, a, st) : launch_forward<D, 0, true, BF, Q8>(p, a, st);
+    }
+    return p.few == 16 ? launch_forward<D, 16, false, BF, Q8>(p, a, st) : launch_forward<D, kFewRows, false, BF, Q8>(p, a, st);
   });
 }
 
