@@ -32,6 +32,7 @@ struct PagedArgs {
   const int *table, *keys, *ends;  // ends: cu_seqlens + 1, or null
   float* part_o;                   // of part p: rows_of_block x D sums, relative to the maximum
   float2* part_ml;                 // of part p: maximum (of exponents of 2) and sum of each row
+  int2* places;                    // of each row of o: its first part's row in these, and how many parts it has
   CacheStrides ks, vs, kss, vss;
   long q_batch, q_seq, q_head, table_stride;  // of q in bytes
   int batch, new_tokens, tokens;              // new_tokens: of each sequence, where ends is null; tokens: in all
@@ -411,6 +412,10 @@ __device__ __forceinline__ void few_rows(const PagedArgs& a, const Part& w, char
     }
   }
 
+  if (a.target && w.p == 0 && threadIdx.x < kRows && row0 + (int)threadIdx.x < rows) {
+    const int row = row0 + threadIdx.x, token = row / a.group, head = w.head * (int)a.group + row - token * (int)a.group;
+    a.places[(w.s.first + token) * a.head + head] = int2{w.number * slot_rows + (int)threadIdx.x, w.parts};
+  }
   // the waves' sums, relative to the largest maximum
 #pragma unroll
   for (int cb = 0; cb < CB; ++cb) {
@@ -829,6 +834,10 @@ __device__ __forceinline__ void many_rows(const PagedArgs& a, const Part& w, cha
   const float f = w.parts > 1 ? 1.f : l_tot == 0.f ? 0.f : 1.f / l_tot;
   char* const stage = smem + wave * (kResident * ManyGeom<D>::kPitch);
   const long slot0 = (long)w.number * kManyRows + wave * kResident;
+  if (z.target && w.p == 0 && lane < kResident && row0w + lane < rows) {
+    const int row = row0w + lane, token = row / z.group, head = w.head * (int)z.group + row - token * (int)z.group;
+    z.places[(w.s.first + token) * z.head + head] = int2{(int)slot0 + lane, w.parts};
+  }
   if (w.parts > 1 && lane < kResident && row0w + lane < rows) z.part_ml[slot0 + lane] = float2{mc, l_tot};
 #pragma unroll
   for (int half = 0; half < D / 64; ++half) {
@@ -886,58 +895,88 @@ __global__ void __launch_bounds__(kPagedThreads, 2) paged_forward_kernel(PagedAr
 }
 
 // ---------------------------------------------------------------------------
-// Rows whose keys went to several parts.  A work group has one row of the output: D / 4 threads to a part's row.
+// Rows whose keys went to several parts.  A slice of D / 4 threads adds up parts of a row, each relative to the largest maximum so
+// far.  A work group has one row, whose parts its slices share, or one for each slice; of those with many parts it then takes
+// one after the other.
 // ---------------------------------------------------------------------------
-template <int D, typename B, bool BF>
-__global__ void __launch_bounds__(256) paged_join_kernel(PagedArgs a) {
-  constexpr int ROWS = B::kMost;
+constexpr int kJoinAhead = 8;  // parts that a slice asks for at a time
+struct Joined {
+  float m, l;
+  f4v x;
+};
+__device__ __forceinline__ void join_in(Joined& r, float m, float l, f4v x, float mx) {
+  const float f = m == -INFINITY ? 0.f : fast_exp2(m - mx);
+  r.l += l * f;  // NaN from a bad page stays
+  r.x += x * f;
+}
+template <int D>
+__device__ __forceinline__ Joined join_parts(const PagedArgs& a, int at, int parts, int first, int step, int slot_rows, int piece) {
+  Joined r{-INFINITY, 0.f, f4v{0.f, 0.f, 0.f, 0.f}};
+  for (int p = first; p < parts; p += kJoinAhead * step) {
+    float2 ml[kJoinAhead];
+    f4v x[kJoinAhead];
+#pragma unroll
+    for (int u = 0; u < kJoinAhead; ++u) {
+      const long row = at + (long)min(p + u * step, parts - 1) * slot_rows;
+      ml[u] = a.part_ml[row];
+      x[u] = *reinterpret_cast<const f4v*>(a.part_o + row * D + piece * 4);
+    }
+    float mx = r.m;
+#pragma unroll
+    for (int u = 0; u < kJoinAhead; ++u)
+      if (p + u * step < parts) mx = fmaxf(mx, ml[u].x);
+    const float f = r.m == -INFINITY ? 0.f : fast_exp2(r.m - mx);
+    r.m = mx, r.l *= f, r.x *= f;
+#pragma unroll
+    for (int u = 0; u < kJoinAhead; ++u)
+      if (p + u * step < parts) join_in(r, ml[u].x, ml[u].y, x[u], mx);
+  }
+  return r;
+}
+
+template <int D, bool BF>
+__global__ void __launch_bounds__(256) paged_join_kernel(PagedArgs a, int slot_rows, int rows_of_group) {
   constexpr int kPieces = D / 4, kSlices = 256 / kPieces;
-  __shared__ f4v sums[kSlices][kPieces];
-  const int lane = threadIdx.x & 63;
-  const int token = (int)blockIdx.x / a.head, head = (int)blockIdx.x - token * a.head;
-  const int b = a.ends ? sequence_of(a.ends, a.batch, token, lane) : token / a.new_tokens;
-  const Sequence s = sequence(a, b);
-  const int i = token - s.first;
-  if (i < 0 || i >= s.n) return;
-  const int per = tiles_of_part<B>(a, lane);
-  const int parts = paged_parts(paged_tiles(s.keys), per);
-  if (parts == 1) return;
-  int before = 0;
-  for (int b0 = lane; b0 < b; b0 += 64) {
-    const Sequence t = sequence(a, b0);
-    before += B::count(t.n * a.group) * paged_parts(paged_tiles(t.keys), per);
+  __shared__ Joined sums[kSlices][kPieces];
+  const int slice = threadIdx.x / kPieces, piece = threadIdx.x % kPieces, rows = a.tokens * a.head;
+  const int room = a.slots * slot_rows;
+  auto place = [&](int row) __attribute__((always_inline)) {
+    if (row >= rows) return int2{0, 1};
+    if (a.ends) {
+      const int token = row / a.head;
+      if (token < a.ends[-1] || token >= a.ends[a.batch - 1]) return int2{0, 1};
+    }
+    int2 r = a.places[row];
+    // of tokens that ranges which make no sense left out it says anything
+    if (r.x < 0 || r.y < 1 || r.x >= room || r.y > (room - 1 - r.x) / slot_rows + 1) r.y = 1;
+    return r;
+  };
+  auto store = [&](int row, const Joined& r) __attribute__((always_inline)) {
+    store4<BF>(a.o + ((long)row * D + piece * 4) * 2, r.x * (r.l == 0.f ? 0.f : 1.f / r.l));
+  };
+  const int row0 = blockIdx.x * rows_of_group;
+  if (rows_of_group > 1) {
+    const int2 mine = place(row0 + slice);
+    if (!__syncthreads_or(mine.y > 2 * kJoinAhead)) {
+      if (mine.y > 1) store(row0 + slice, join_parts<D>(a, mine.x, mine.y, 0, 1, slot_rows, piece));
+      return;
+    }
   }
-  before = (int)sum_over_wave(before);
-  const int kvh = head / a.group, row = i * a.group + head - kvh * a.group;
-  const int rows_of_block = B::rows_of_block(s.n * a.group), block = row / rows_of_block;
-  const long first = (long)before * a.kv_head + ((long)kvh * B::count(s.n * a.group) + block) * parts;
-  if (first + parts > a.slots) return;
-  const long at = first * ROWS + row % rows_of_block;
-  float mx = -INFINITY;
-  for (int p = lane; p < parts; p += 64) mx = fmaxf(mx, a.part_ml[at + (long)p * ROWS].x);
+  for (int u = 0; u < rows_of_group; ++u) {
+    const int2 at = place(row0 + u);
+    if (at.y == 1) continue;
+    __syncthreads();
+    sums[slice][piece] = join_parts<D>(a, at.x, at.y, slice, kSlices, slot_rows, piece);
+    __syncthreads();
+    if (slice) continue;
+    float mx = -INFINITY;
 #pragma unroll
-  for (int d = 1; d < 64; d *= 2) mx = fmaxf(mx, __shfl_xor(mx, d));
-  float sum = 0.f;
-  for (int p = lane; p < parts; p += 64) {
-    const float2 ml = a.part_ml[at + (long)p * ROWS];
-    sum += ml.x == -INFINITY ? ml.y : ml.y * fast_exp2(ml.x - mx);
+    for (int v = 0; v < kSlices; ++v) mx = fmaxf(mx, sums[v][piece].m);
+    Joined r{mx, 0.f, f4v{0.f, 0.f, 0.f, 0.f}};
+#pragma unroll
+    for (int v = 0; v < kSlices; ++v) join_in(r, sums[v][piece].m, sums[v][piece].l, sums[v][piece].x, mx);
+    store(row0 + u, r);
   }
-#pragma unroll
-  for (int d = 1; d < 64; d *= 2) sum += __shfl_xor(sum, d);
-  const int slice = threadIdx.x / kPieces, piece = threadIdx.x % kPieces;
-  f4v x = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll 4
-  for (int p = slice; p < parts; p += kSlices) {
-    const float m = a.part_ml[at + (long)p * ROWS].x;
-    const f4v y = *reinterpret_cast<const f4v*>(a.part_o + (at + (long)p * ROWS) * D + piece * 4);
-    x += y * (m == -INFINITY ? 0.f : fast_exp2(m - mx));
-  }
-  sums[slice][piece] = x;
-  __syncthreads();
-  if (slice) return;
-#pragma unroll
-  for (int v = 1; v < kSlices; ++v) x += sums[v][piece];
-  store4<BF>(a.o + (((long)token * a.head + head) * D + piece * 4) * 2, x * (sum == 0.f ? 0.f : 1.f / sum));
 }
 
 // ---------------------------------------------------------------------------
@@ -1078,9 +1117,9 @@ __global__ void __launch_bounds__(256) paged_read_kernel(ReadArgs a) {
 // ---------------------------------------------------------------------------
 // Host.
 // ---------------------------------------------------------------------------
-template <typename Args>
-hipError_t launch(void (*kernel)(Args), dim3 grid, unsigned block, hipStream_t stream, Args args) {
-  void* ptrs[] = {&args};
+template <typename... Args>
+hipError_t launch(void (*kernel)(Args...), dim3 grid, unsigned block, hipStream_t stream, Args... args) {
+  void* ptrs[] = {&args...};
   return hipLaunchKernel((const void*)kernel, grid, dim3(block), ptrs, 0, stream);
 }
 
@@ -1150,14 +1189,18 @@ Launch plan(const paged_mha_cache* c, const paged_mha_batch* b, int head, int ma
   p.target = (long)b->table_width * c->page_size > kLeast * kPagedTile ? kTarget : 0;
   return p;
 }
-size_t workspace_bytes_of(const Launch& p, int d) { return (size_t)p.slots() * p.slot_rows() * (d * 4 + 8); }
+// Sums of the parts' rows, their maxima and totals, where each row of o has its parts.
+size_t workspace_bytes_of(const Launch& p, int d, long rows) {
+  return p.target ? (size_t)p.slots() * p.slot_rows() * (d * 4 + 8) + (size_t)rows * 8 : 0;
+}
 
 template <int D, int FEW, bool MANY, bool BF, bool Q8>
 int launch_forward(const Launch& p, const PagedArgs& a, hipStream_t stream) {
   if (launch(paged_forward_kernel<D, FEW, MANY, BF, Q8>, dim3(p.grid()), kPagedThreads, stream, a) != hipSuccess) return FUSED_MHA_ERR_LAUNCH;
   if (!p.target) return FUSED_MHA_OK;
-  const long rows = (long)a.tokens * a.head;
-  return launch(paged_join_kernel<D, Blocks<FEW, MANY>, BF>, dim3(rows), 256, stream, a) == hipSuccess ? FUSED_MHA_OK : FUSED_MHA_ERR_LAUNCH;
+  const int rows = a.tokens * a.head, rows_of_group = MANY ? 256 / (D / 4) : 1;
+  return launch(paged_join_kernel<D, BF>, dim3((rows + rows_of_group - 1) / rows_of_group), 256, stream, a, p.slot_rows(), rows_of_group) == hipSuccess
+             ? FUSED_MHA_OK : FUSED_MHA_ERR_LAUNCH;
 }
 
 // f(D, BF, Q8) with the values of a cache as constants.
@@ -1232,11 +1275,12 @@ static int check_forward(const paged_mha_cache* c, const paged_mha_batch* b, int
   if (head <= 0 || max_new < 0) return FUSED_MHA_ERR_BAD_SHAPE;
   if (head % c->kv_head) return PAGED_MHA_ERR_BAD_GROUP;
   if (head > (1 << 16) || all_tokens(b) * head >= (1L << 30)) return FUSED_MHA_ERR_TOO_LARGE;
-  return plan(c, b, head, max_new).grid() >= (1L << 30) ? FUSED_MHA_ERR_TOO_LARGE : FUSED_MHA_OK;
+  const Launch p = plan(c, b, head, max_new);
+  return p.grid() >= (1L << 30) || p.slots() * p.slot_rows() >= (1L << 30) ? FUSED_MHA_ERR_TOO_LARGE : FUSED_MHA_OK;
 }
 
 size_t paged_mha_forward_workspace_bytes(const paged_mha_cache* c, const paged_mha_batch* b, int head, int max_new) {
-  return check_forward(c, b, head, max_new) ? 0 : workspace_bytes_of(plan(c, b, head, max_new), c->d);
+  return check_forward(c, b, head, max_new) ? 0 : workspace_bytes_of(plan(c, b, head, max_new), c->d, all_tokens(b) * head);
 }
 
 int paged_mha_forward(const paged_mha_cache* c, const paged_mha_batch* b, const void* q, const fused_mha_strides* q_st, void* o,
@@ -1247,7 +1291,7 @@ int paged_mha_forward(const paged_mha_cache* c, const paged_mha_batch* b, const 
   if (!isfinite(scale)) return FUSED_MHA_ERR_BAD_SCALE;
   if (bad_strides(q_st)) return FUSED_MHA_ERR_BAD_STRIDE;
   const Launch p = plan(c, b, head, max_new);
-  const size_t wanted = workspace_bytes_of(p, c->d);
+  const size_t wanted = workspace_bytes_of(p, c->d, all_tokens(b) * head);
   if (wanted && !workspace) return FUSED_MHA_ERR_NULL_POINTER;
   if (workspace_bytes < wanted) return PAGED_MHA_ERR_WORKSPACE;
   if (misaligned(q) || misaligned(o) || misaligned(workspace)) return FUSED_MHA_ERR_MISALIGNED;
@@ -1258,6 +1302,7 @@ int paged_mha_forward(const paged_mha_cache* c, const paged_mha_batch* b, const 
   a.table = b->page_table, a.keys = b->cache_seqlens, a.ends = b->cu_seqlens ? b->cu_seqlens + 1 : nullptr;
   a.part_o = (float*)workspace;
   a.part_ml = (float2*)((char*)workspace + (size_t)p.slots() * p.slot_rows() * c->d * 4);
+  a.places = (int2*)(a.part_ml + (size_t)p.slots() * p.slot_rows());
   a.ks = in_bytes(c->key_strides, bytes), a.vs = in_bytes(c->value_strides, bytes);
   a.kss = in_bytes(c->key_scale_strides, 1), a.vss = in_bytes(c->value_scale_strides, 1);
   a.q_batch = a.ends ? 0 : q_st->batch * 2, a.q_seq = q_st->seq * 2, a.q_head = q_st->head * 2;
