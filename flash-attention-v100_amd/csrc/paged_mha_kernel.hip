@@ -247,12 +247,12 @@ struct FewGeom {
 };
 
 template <int D, int CB, bool BF, bool Q8>
-__device__ __forceinline__ void few_rows(const PagedArgs& a, const Part& w, char* smem, float2* joined, int slot_rows) {
+__device__ __forceinline__ void few_rows(const PagedArgs& a, const Part& w, char* smem, int slot_rows) {
   using T = SwzTile<D>;
   using G = FewGeom<D, CB>;
   constexpr int kRows = G::kRows, kNC = T::kNC, kKS = D / 32, kDB = D / 16;
   constexpr int kLoads = Q8 ? kNC / 2 : kNC;  // of 16 positions: 64 bytes of each
-  float2(*const join)[kRows] = reinterpret_cast<float2(*)[kRows]>(joined);
+  float2(*const join)[kRows] = reinterpret_cast<float2(*)[kRows]>(smem + kFewWaves * G::kWaveBytes);
 
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int m = lane & 15, g = lane >> 4;
@@ -468,11 +468,13 @@ __device__ __forceinline__ void few_rows(const PagedArgs& a, const Part& w, char
 // instructions, the running maximum raised only where a tile's probabilities come out too large.  New tokens stand anywhere
 // against the tiles, so up to two tiles of a wave need a mask; they are done after the main loop.
 // ---------------------------------------------------------------------------
-template <int D>
+template <int D, bool Q8>
 struct ManyGeom {
   static constexpr int kPitch = 64 * 4 + 16;  // of a row of 64 sums in LDS
   static constexpr int kTileBytes = 4 * SwzTile<D>::kBytes, kStageBytes = kPagedThreads / 64 * kResident * kPitch;
-  static constexpr int kBytes = kTileBytes > kStageBytes ? kTileBytes : kStageBytes;
+  static constexpr int kFlags = kTileBytes > kStageBytes ? kTileBytes : kStageBytes;  // where the waves say that a page is bad
+  static constexpr int kRaw = 16 * D;  // bytes of 16 rows in 8 bits
+  static constexpr int kBytes = Q8 ? kFlags + kPagedThreads / 64 * 2 * kRaw : kFlags + 16;
 };
 constexpr float kNoMaximum = -3.4028234663852886e38f;  // in the place of -inf: a difference of two of them is 0
 
@@ -489,8 +491,9 @@ __device__ __forceinline__ unsigned pack2_here(float x, float y) {
   return r;
 }
 
-template <int D, bool BF>
-__device__ __forceinline__ void many_rows(const PagedArgs& a, const Part& w, char* smem, int* bad_pages) {
+template <int D, bool BF, bool Q8>
+__device__ __forceinline__ void many_rows(const PagedArgs& a, const Part& w, char* smem) {
+  using M = ManyGeom<D, Q8>;
   using G = TileGeom<D>;
   using T = SwzTile<D>;
   constexpr int kDB = G::kDBlocks, kIPW = T::kNC;  // copies of a wave and tile: 16 rows, 64 bytes of each
@@ -518,7 +521,7 @@ __device__ __forceinline__ void many_rows(const PagedArgs& a, const Part& w, cha
   const char* const v_head = a.v + (long)w.head * a.vs.head;
   const int last_stretch = (w.s.keys - 1) >> 4;
   const int k_shift = a.k_shift, v_shift = a.v_shift;
-  unsigned k_at = 0, v_at = 0;
+  unsigned k_at = 0, v_at = 0, ks_at = 0, vs_at = 0;
   int at_from = 0;
   bool bad = w.s.past;
   auto fetch_at = [&](int j) __attribute__((always_inline)) {
@@ -533,18 +536,22 @@ __device__ __forceinline__ void many_rows(const PagedArgs& a, const Part& w, cha
     k_at = (unsigned)((id * a.ks.page + (long)slot * a.ks.slot) >> a.k_shift);
     v_at = (unsigned)((id * a.vs.page + (long)slot * a.vs.slot) >> a.v_shift);
     asm volatile("" : "+v"(k_at), "+v"(v_at));
+    if constexpr (Q8) {
+      ks_at = (unsigned)(id * a.kss.page + (long)slot * a.kss.slot);
+      vs_at = (unsigned)(id * a.vss.page + (long)slot * a.vss.slot);
+      asm volatile("" : "+v"(ks_at), "+v"(vs_at));
+    }
   };
-  constexpr int kBack = 960 * (kIPW - 1);  // see copy16_blocks
+  constexpr int kCopies = Q8 ? kIPW / 2 : kIPW, kBack = 960 * (kCopies - 1);  // see copy16_blocks
   int k_goff, v_goff;
   {
-    const int lane = lane_now(), r16 = lane >> 2, col = ((lane & 3) ^ swz(r16 >> 2)) * 16;
+    const int lane = lane_now(), r16 = lane >> 2, col = (Q8 ? lane & 3 : (lane & 3) ^ swz(r16 >> 2)) * 16;
     k_goff = r16 * a.ks.slot + col + kBack;
     v_goff = r16 * a.vs.slot + col + kBack;
     asm volatile("" : "+v"(k_goff), "+v"(v_goff));
   }
   const unsigned lds0 = (unsigned)(uintptr_t)(__attribute__((address_space(3))) char*)smem;
   const unsigned lds_w = lds0 + wave * (kIPW * 1024);
-  // K(j) and V(j - 2) are asked for in the same step: V comes out of the same registers two tiles later, before they are fetched anew
   auto past_end = [&](int j, int off, bool value) __attribute__((always_inline)) {  // rows behind the last key: that one
     const PagedArgs a = args_again();
     const int stride = value ? a.vs.slot : a.ks.slot;
@@ -553,17 +560,49 @@ __device__ __forceinline__ void many_rows(const PagedArgs& a, const Part& w, cha
     return off - max(r16 - (w.s.keys - 1 - stretch * 16), 0) * stride;
   };
   const int j_end = (w.s.keys - 1) / kPagedTile - t0;  // the tile with the last key
-  auto copy_k = [&](int j, int slot) __attribute__((always_inline)) {
-    const char* const from = k_head + ((long)(unsigned)__builtin_amdgcn_readlane(k_at, j - at_from) << k_shift) - kBack;
-    int off = k_goff;
-    if (j == j_end) off = past_end(j, off, false);
-    copy16_blocks<kIPW>(wave_uniform(from), off, __builtin_amdgcn_readfirstlane(lds_w + slot * T::kBytes));
+  // 64 bytes of 16 rows to each 1 KiB from `to` on
+  auto copy = [&](const char* head, unsigned at, int shift, int off, int j, bool value, unsigned to) __attribute__((always_inline)) {
+    const char* const from = head + ((long)(unsigned)__builtin_amdgcn_readlane(at, j - at_from) << shift) - kBack;
+    if (j == j_end) off = past_end(j, off, value);
+    if constexpr (kCopies == 1) copy16(wave_uniform(from), off, smem + __builtin_amdgcn_readfirstlane(to - lds0));
+    else copy16_blocks<kCopies>(wave_uniform(from), off, __builtin_amdgcn_readfirstlane(to));
   };
-  auto copy_v = [&](int j, int slot) __attribute__((always_inline)) {
-    const char* const from = v_head + ((long)(unsigned)__builtin_amdgcn_readlane(v_at, j - at_from) << v_shift) - kBack;
-    int off = v_goff;
-    if (j == j_end) off = past_end(j, off, true);
-    copy16_blocks<kIPW>(wave_uniform(from), off, __builtin_amdgcn_readfirstlane(lds_w + kVOff + slot * T::kBytes));
+  auto copy_k = [&](int j, unsigned to) __attribute__((always_inline)) { copy(k_head, k_at, k_shift, k_goff, j, false, to); };
+  auto copy_v = [&](int j, unsigned to) __attribute__((always_inline)) { copy(v_head, v_at, v_shift, v_goff, j, true, to); };
+  // A cache in 8 bits: rows come to LDS as they are, to a place of the wave's own, with their scales in registers, and go from there
+  // to the tile a step later.
+  const unsigned raw_k = lds0 + M::kFlags + wave * 2 * M::kRaw, raw_v = raw_k + M::kRaw;
+  unsigned k_sc = 0, v_sc = 0;
+  auto scale_from = [&](const unsigned char* scales, unsigned at, int j, bool value) __attribute__((always_inline)) -> unsigned {
+    const PagedArgs a = args_again();
+    const CacheStrides st = value ? a.vss : a.kss;
+    const int r16 = min(lane_now() >> 2, w.s.keys - 1 - min(4 * (t0 + j) + wave, last_stretch) * 16);
+    const unsigned char* const from = scales + (long)w.head * st.head + (unsigned)__builtin_amdgcn_readlane(at, j - at_from);
+    return from[(unsigned)(r16 * st.slot)];
+  };
+  auto ask_k = [&](int j, unsigned to, unsigned& sc) __attribute__((always_inline)) {
+    copy_k(j, to);
+    sc = scale_from(args_again().k_scale, ks_at, j, false);
+  };
+  auto ask_v = [&](int j) __attribute__((always_inline)) {
+    copy_v(j, raw_v);
+    v_sc = scale_from(args_again().v_scale, vs_at, j, true);
+  };
+  // Of a lane's 16 values one half is chunk c, the other c ^ 1 of a row; lanes two apart write the same banks, so they begin with
+  // different halves.
+  auto put = [&](unsigned raw, unsigned sc, unsigned tile) __attribute__((always_inline)) {
+    typedef __attribute__((address_space(3))) u2v lds_u2v;
+    typedef __attribute__((address_space(3))) u4v lds_u4v;
+    const int lane = lane_now(), r16 = lane >> 2, q4 = lane & 3, half = q4 >> 1;
+    const unsigned from = raw + lane * 16 + half * 8;
+    const unsigned to = tile + T::block_off(wave, half) + r16 * 64 + (((2 * (q4 & 1) + half) ^ swz(r16 >> 2)) * 16);
+    const float scale = scale_of(sc);
+#pragma unroll
+    for (int i = 0; i < kCopies; ++i) {
+      const u2v x = *(const lds_u2v*)(uintptr_t)(from + 1024 * i), y = *(const lds_u2v*)(uintptr_t)((from ^ 8) + 1024 * i);
+      *(lds_u4v*)(uintptr_t)(to + T::block_off(0, 2 * i)) = from_e4m3<BF>(x[0], x[1], scale);
+      *(lds_u4v*)(uintptr_t)((to ^ 16) + T::block_off(0, 2 * i)) = from_e4m3<BF>(y[0], y[1], scale);
+    }
   };
 
   // the block's rows of q fill the slots of V, which comes later
@@ -582,8 +621,21 @@ __device__ __forceinline__ void many_rows(const PagedArgs& a, const Part& w, cha
   }
   if (nt > 0) {
     fetch_at(0);
-    copy_k(0, 0);
-    if (nt > 1) copy_k(1, 1);
+    if constexpr (Q8) {
+      unsigned k_sc1 = 0;
+      ask_k(0, raw_k, k_sc);
+      if (nt > 1) ask_k(1, raw_v, k_sc1);
+      wait_vm<0>();
+      asm volatile("" ::: "memory");
+      put(raw_k, k_sc, lds0);
+      if (nt > 1) put(raw_v, k_sc1, lds0 + T::kBytes);
+      staged_rows_read();
+      if (nt > 2) ask_k(2, raw_k, k_sc);
+      ask_v(0);
+    } else {
+      copy_k(0, lds_w);
+      if (nt > 1) copy_k(1, lds_w + T::kBytes);
+    }
   }
   h8 qf[G::kKSteps];
   {
@@ -692,18 +744,38 @@ __device__ __forceinline__ void many_rows(const PagedArgs& a, const Part& w, cha
       __builtin_amdgcn_sched_barrier(0);
     }
   };
-  // Step j uses K(j + 1) and V(j - 1), both in slot (j + 1) & 1; K(j + 2) and V(j) are copied into the other one.
+  // Step j uses K(j + 1) and V(j - 1), both in slot (j + 1) & 1; K(j + 2) and V(j) are copied into the other one.  Out of 8 bits
+  // they go there now, and K(j + 3) and V(j + 1) are asked for.
   auto top_wait = [&]() __attribute__((always_inline)) {
     wait_vm<0>();
     block_barrier();
   };
   auto fetch_for = [&](int j) __attribute__((always_inline)) {  // the registers hold tiles at_from .. at_from + 63
-    if (j + 2 - at_from >= 64 && j < nt) fetch_at(j);
+    if (j + (Q8 ? 3 : 2) - at_from >= 64 && j < nt) fetch_at(j);
+  };
+  auto next_k = [&](int j, int slot) __attribute__((always_inline)) {
+    if constexpr (Q8) {
+      if (j + 2 < nt) put(raw_k, k_sc, lds0 + slot * T::kBytes);
+    } else {
+      if (j + 2 < nt) copy_k(j + 2, lds_w + slot * T::kBytes);
+    }
+  };
+  auto next_v = [&](int j, int slot) __attribute__((always_inline)) {
+    if constexpr (Q8) put(raw_v, v_sc, lds0 + kVOff + slot * T::kBytes);
+    else copy_v(j, lds_w + kVOff + slot * T::kBytes);
+  };
+  auto ask = [&](int j) __attribute__((always_inline)) {
+    if constexpr (Q8) {
+      staged_rows_read();  // what lies there has been read
+      if (j + 3 < nt) ask_k(j + 3, raw_k, k_sc);
+      if (j + 1 < nt) ask_v(j + 1);
+    }
   };
   auto top_copy = [&](int j, int slot) __attribute__((always_inline)) {
     fetch_for(j);
-    if (j + 2 < nt) copy_k(j + 2, slot);
-    if (j < nt) copy_v(j, slot);
+    next_k(j, slot);
+    if (j < nt) next_v(j, slot);
+    ask(j);
   };
   auto step = [&](int j, auto slot_tag, const f16v (&s)[2], f16v (&sn)[2]) __attribute__((always_inline)) {
     constexpr int kSlot = decltype(slot_tag)::value;  // (j + 1) & 1
@@ -730,15 +802,20 @@ __device__ __forceinline__ void many_rows(const PagedArgs& a, const Part& w, cha
     };
     top_wait();
     fetch_for(j);
+    if constexpr (Q8) {
+      next_v(j, 1 - kSlot);
+      next_k(j, 1 - kSlot);
+      ask(j);
+    }
 #pragma unroll
     for (int m = 0; m < kLead; ++m) frag[m] = read(m);
-    constexpr int kCopyKAt = D == 128 ? 8 : 0;  // K's copies follow when V's are through
-    copy_v(j, 1 - kSlot);
-    if (kCopyKAt == 0 && j + 2 < nt) copy_k(j + 2, 1 - kSlot);
+    constexpr int kCopyKAt = Q8 ? -1 : D == 128 ? 8 : 0;  // K's copies follow when V's are through
+    if (!Q8) next_v(j, 1 - kSlot);
+    if (kCopyKAt == 0) next_k(j, 1 - kSlot);
     __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
     for (int m = 0; m < kM + 2; ++m) {
-      if (kCopyKAt != 0 && m == kCopyKAt && j + 2 < nt) copy_k(j + 2, 1 - kSlot);
+      if (kCopyKAt != 0 && m == kCopyKAt) next_k(j, 1 - kSlot);
       if (m < kM && m % 2 == 0) {  // one wait for the fragments of this unit and the next
         if (D == 64) wait_lds_pinned(reads(m + 2));
         else wait_lds(reads(m + 2));
@@ -768,8 +845,10 @@ __device__ __forceinline__ void many_rows(const PagedArgs& a, const Part& w, cha
     return l0 + l1;
   };
 
-  if (nt > 1) wait_vm<kIPW>();  // the second tile of K may still be on its way
-  else wait_vm<0>();
+  if (!Q8) {
+    if (nt > 1) wait_vm<kIPW>();  // the second tile of K may still be on its way
+    else wait_vm<0>();
+  }
   block_barrier();
   if (ntw > 0) scores(0, sA);
   int j = 0;
@@ -825,6 +904,7 @@ __device__ __forceinline__ void many_rows(const PagedArgs& a, const Part& w, cha
     }
   }
 
+  int* const bad_pages = reinterpret_cast<int*>(smem + M::kFlags);
   bad_pages[wave] = bad;  // each wave has looked at a quarter of the pages
   block_barrier();        // every wave is done with the rings: they become the staging tiles
   const PagedArgs z = args_again();
@@ -832,7 +912,7 @@ __device__ __forceinline__ void many_rows(const PagedArgs& a, const Part& w, cha
   float l_tot = l_run + other_half(l_run);
   if (bad_pages[0] | bad_pages[1] | bad_pages[2] | bad_pages[3]) l_tot = NAN;
   const float f = w.parts > 1 ? 1.f : l_tot == 0.f ? 0.f : 1.f / l_tot;
-  char* const stage = smem + wave * (kResident * ManyGeom<D>::kPitch);
+  char* const stage = smem + wave * (kResident * M::kPitch);
   const long slot0 = (long)w.number * kManyRows + wave * kResident;
   if (z.target && w.p == 0 && lane < kResident && row0w + lane < rows) {
     const int row = row0w + lane, token = row / z.group, head = w.head * (int)z.group + row - token * (int)z.group;
@@ -848,14 +928,14 @@ __device__ __forceinline__ void many_rows(const PagedArgs& a, const Part& w, cha
         f4v x;
 #pragma unroll
         for (int r = 0; r < 4; ++r) x[r] = o[2 * half + db][4 * e + r] * f;
-        *reinterpret_cast<f4v*>(stage + (lane & 31) * ManyGeom<D>::kPitch + (db * 32 + 8 * e + 4 * (lane >> 5)) * 4) = x;
+        *reinterpret_cast<f4v*>(stage + (lane & 31) * M::kPitch + (db * 32 + 8 * e + 4 * (lane >> 5)) * 4) = x;
       }
     __builtin_amdgcn_s_waitcnt(0xC07F);  // lgkmcnt(0): the wave's own writes have landed
     asm volatile("" ::: "memory");
 #pragma unroll
     for (int pass = 0; pass < kResident / 4; ++pass) {
       const int r = 4 * pass + (lane >> 4), row = row0w + r, piece = lane & 15;
-      const f4v x = *reinterpret_cast<const f4v*>(stage + r * ManyGeom<D>::kPitch + piece * 16);
+      const f4v x = *reinterpret_cast<const f4v*>(stage + r * M::kPitch + piece * 16);
       if (row < rows) {
         if (w.parts > 1) {
           *reinterpret_cast<f4v*>(z.part_o + (slot0 + r) * D + half * 64 + piece * 4) = x;
@@ -876,10 +956,9 @@ __device__ __forceinline__ void many_rows(const PagedArgs& a, const Part& w, cha
 template <int D, int FEW, bool MANY, bool BF, bool Q8>
 __global__ void __launch_bounds__(kPagedThreads, 2) paged_forward_kernel(PagedArgs a) {
   using B = Blocks<FEW, MANY>;
-  constexpr int kFewBytes = FEW ? kFewWaves * FewGeom<D, FEW ? FEW / 16 : 1>::kWaveBytes : 0, kManyBytes = MANY ? ManyGeom<D>::kBytes : 0;
+  constexpr int kFewBytes = FEW ? kFewWaves * (FewGeom<D, FEW ? FEW / 16 : 1>::kWaveBytes + FEW * (int)sizeof(float2)) : 0;
+  constexpr int kManyBytes = MANY ? ManyGeom<D, Q8>::kBytes : 0;
   __shared__ __attribute__((aligned(1024))) char smem[kFewBytes > kManyBytes ? kFewBytes : kManyBytes];
-  __shared__ float2 joined[FEW ? kFewWaves * FEW : 1];
-  __shared__ int bad_pages[kFewWaves];
   if (a.zero_rest) {
     const int rest = min(max(a.ends[a.batch - 1], 0), a.tokens);
     const long from = (long)rest * a.head * D * 2, to = (long)a.tokens * a.head * D * 2;
@@ -889,9 +968,9 @@ __global__ void __launch_bounds__(kPagedThreads, 2) paged_forward_kernel(PagedAr
   const Part w = part_of<B>(a, blockIdx.x, threadIdx.x & 63);
   if (w.b < 0) return;
   if constexpr (MANY) {
-    if (B::many(w.s.n * a.group)) return many_rows<D, BF>(a, w, smem, bad_pages);
+    if (B::many(w.s.n * a.group)) return many_rows<D, BF, Q8>(a, w, smem);
   }
-  if constexpr (FEW != 0) few_rows<D, FEW / 16, BF, Q8>(a, w, smem, joined, B::kMost);
+  if constexpr (FEW != 0) few_rows<D, FEW / 16, BF, Q8>(a, w, smem, B::kMost);
 }
 
 // ---------------------------------------------------------------------------
@@ -1179,9 +1258,13 @@ bool fits(const paged_mha_cache* c, const paged_mha_strides& s, int bytes, int& 
 Launch plan(const paged_mha_cache* c, const paged_mha_batch* b, int head, int max_new) {
   const long group = head / c->kv_head;
   const long most = (b->cu_seqlens && max_new > 0 ? std::min(max_new, b->tokens) : b->tokens) * group;
+  const bool q8 = c->cache_type == PAGED_MHA_E4M3;
   int shift;
+  auto all_fit = [&](const paged_mha_strides& s) { return fits(c, s, q8 ? 1 : 2, shift); };
+  auto scales_fit = [&](const paged_mha_strides& s) { return s.page * (c->pages - 1) + s.slot * c->page_size < (1LL << 32); };
   Launch p;
-  p.many = most > kFewRows && c->cache_type == c->type && fits(c, c->key_strides, 2, shift) && fits(c, c->value_strides, 2, shift);
+  p.many = most > kFewRows && all_fit(c->key_strides) && all_fit(c->value_strides) &&
+           (!q8 || (scales_fit(c->key_scale_strides) && scales_fit(c->value_scale_strides)));
   p.few = most <= 16 ? 16 : !p.many || b->cu_seqlens ? kFewRows : 0;
   const int least_rows = p.few ? p.few : kManyRows;
   const long blocks = b->cu_seqlens ? b->tokens * group / least_rows + b->batch : b->batch * ((b->tokens * group + least_rows - 1) / least_rows);
@@ -1313,14 +1396,12 @@ int paged_mha_forward(const paged_mha_cache* c, const paged_mha_batch* b, const 
   a.c = scale * kLog2e;
   a.causal = causal != 0, a.zero_rest = zero_rest != 0 && a.ends;
   a.target = p.target, a.least = kLeast, a.slots = (int)p.slots();
-  if (p.many) fits(c, c->key_strides, 2, a.k_shift), fits(c, c->value_strides, 2, a.v_shift);
+  if (p.many) fits(c, c->key_strides, bytes, a.k_shift), fits(c, c->value_strides, bytes, a.v_shift);
   return with_types(c, [&](auto d, auto bf, auto q8) {
     constexpr int D = decltype(d)::value;
     constexpr bool BF = decltype(bf)::value != 0, Q8 = decltype(q8)::value != 0;
     const hipStream_t st = (hipStream_t)stream;
-    if constexpr (!Q8) {
-      if (p.many) return p.few ? launch_forward<D, kFewRows, true, BF, Q8>(p, a, st) : launch_forward<D, 0, true, BF, Q8>(p, a, st);
-    }
+    if (p.many) return p.few ? launch_forward<D, kFewRows, true, BF, Q8>(p, a, st) : launch_forward<D, 0, true, BF, Q8>(p, a, st);
     return p.few == 16 ? launch_forward<D, 16, false, BF, Q8>(p, a, st) : launch_forward<D, kFewRows, false, BF, Q8>(p, a, st);
   });
 }
