@@ -30,9 +30,9 @@ struct PagedArgs {
   const unsigned char *k_scale, *v_scale;
   char* o;
   const int *table, *keys, *ends;  // ends: cu_seqlens + 1, or null
-  float* part_o;                   // of part p: rows_of_block x D sums, relative to the maximum
-  float2* part_ml;                 // of part p: maximum (of exponents of 2) and sum of each row
-  int2* places;                    // of each row of o: its first part's row in these, and how many parts it has
+  float* part_o;                   // of each place (paged_place): a block's rows x D sums, relative to the maximum
+  float2* part_ml;                 // maximum (of exponents of 2) and sum of each row
+  int2* places;                    // of each row of o: its row in place 2 r if its item begins in stretch r, and how many parts it has
   CacheStrides ks, vs, kss, vss;
   long q_batch, q_seq, q_head, table_stride;  // of q in bytes
   int batch, new_tokens, tokens;              // new_tokens: of each sequence, where ends is null; tokens: in all
@@ -40,8 +40,8 @@ struct PagedArgs {
   FmhaDivisor group, page_size;  // group: query heads of a key head
   float c;                       // scale * log2(e)
   int causal, zero_rest;
-  int target, least;  // parts aimed at and their least tiles; target 0: an item is a part
-  int slots;          // parts there is room for: enough unless entries of ends go back
+  int shared;   // items are shared out (paged_plan.h), otherwise each has a work group
+  int step[2];  // of PagedLine under causal masking, for blocks of few rows and of many
   int k_shift, v_shift;  // offsets of 16 positions in the cache are multiples of 2^shift bytes, fewer than 2^32
 };
 
@@ -62,10 +62,11 @@ __device__ __forceinline__ PagedArgs args_again() {
 struct Sequence {
   int first, n;  // its tokens
   int keys;
-  bool past;     // it has more keys than the page table has places
+  int past;      // it has more keys than the page table has places
 };
 __device__ __forceinline__ Sequence sequence(const PagedArgs& a, int b) {
   Sequence s;
+  const int keys = max(a.keys[b], 0);
   if (a.ends) {
     const int lo = a.ends[b - 1], hi = a.ends[b];
     s.first = min(max(lo, 0), a.tokens);
@@ -74,10 +75,9 @@ __device__ __forceinline__ Sequence sequence(const PagedArgs& a, int b) {
     s.first = b * a.new_tokens;
     s.n = a.new_tokens;
   }
-  const int keys = max(a.keys[b], 0);
-  const long places = (long)a.width * (int)a.page_size;
+  const int places = a.width * (int)a.page_size;  // below 2^30
   s.past = keys > places;
-  s.keys = s.past ? (int)places : keys;
+  s.keys = min(keys, places);
   return s;
 }
 
@@ -102,17 +102,25 @@ __device__ __forceinline__ const half_t* wave_uniform(const char* p) {
   return (const half_t*)(((uintptr_t)hi << 32) | lo);
 }
 
-__device__ __forceinline__ long sum_over_wave(long x) {
-#pragma unroll
-  for (int d = 1; d < 64; d *= 2) x += __shfl_xor(x, d);
-  return x;
+// The value of one lane.
+__device__ __forceinline__ long of_lane(long x, int lane) {
+  const unsigned lo = __builtin_amdgcn_readlane((unsigned)x, lane), hi = __builtin_amdgcn_readlane((unsigned)((unsigned long)x >> 32), lane);
+  return (long)(((unsigned long)hi << 32) | lo);
 }
-__device__ __forceinline__ int scan_over_wave(int x, int lane) {  // with its own
-#pragma unroll
-  for (int d = 1; d < 64; d *= 2) {
-    const int y = __shfl_up(x, d);
-    if (lane >= d) x += y;
-  }
+// The sum over lanes 0 .. the lane's own, by moves inside rows of 16 lanes and of the last lane of a row, or of two, to the next.
+template <int kMove, int kRows>
+__device__ __forceinline__ long moved(long x) {
+  const unsigned lo = __builtin_amdgcn_update_dpp(0, (int)x, kMove, kRows, 15, false);
+  const unsigned hi = __builtin_amdgcn_update_dpp(0, (int)((unsigned long)x >> 32), kMove, kRows, 15, false);
+  return (long)(((unsigned long)hi << 32) | lo);
+}
+__device__ __forceinline__ long scan_over_wave(long x) {
+  x += moved<0x111, 15>(x);
+  x += moved<0x112, 15>(x);
+  x += moved<0x114, 15>(x);
+  x += moved<0x118, 15>(x);
+  x += moved<0x142, 10>(x);  // lane 15 of rows 0 and 2 to rows 1 and 3
+  x += moved<0x143, 12>(x);  // lane 31 to rows 2 and 3
   return x;
 }
 
@@ -127,63 +135,84 @@ struct Blocks {
   static __device__ __forceinline__ int count(int rows) { return paged_blocks(rows, rows_of_block(rows)); }
 };
 
-// Tiles of a part.
-template <typename B>
-__device__ __forceinline__ int tiles_of_part(const PagedArgs& a, int lane) {
-  if (a.target == 0) return 1 << 30;
-  long tiles = 0;
-  for (int b = lane; b < a.batch; b += 64) {
-    const Sequence s = sequence(a, b);
-    tiles += (long)B::count(s.n * a.group) * paged_tiles(s.keys);
-  }
-  return __builtin_amdgcn_readfirstlane(paged_tiles_of_part(sum_over_wave(tiles) * a.kv_head, a.target, a.least));
-}
-
-// The part of work group w, or b = -1.
+// What a work group does of an item.
 struct Part {
-  int b, head, block, p, parts, number;
+  int b, head, block;
+  int t0, t1;        // tiles
+  bool whole;        // the item is not in other stretches too
+  bool opens;        // it begins here
+  int place, parts;  // of the part's sums; of the item
+  int stretch;
   Sequence s;
 };
+
+// The items of a work group's stretch, one after the other; all lanes together.  A lane has one of 64 sequences in its registers.
 template <typename B>
-__device__ __forceinline__ Part part_of(const PagedArgs& a, int w, int lane) {
-  const int per = tiles_of_part<B>(a, lane);
-  auto parts_of = [&](int b) __attribute__((always_inline)) {  // of one key head
-    if (b >= a.batch) return 0;
-    const Sequence s = sequence(a, b);
-    return B::count(s.n * a.group) * paged_parts(paged_tiles(s.keys), per);
-  };
-  Part r;
-  r.b = -1;
-  int all = 0;
-  for (int b0 = 0; b0 < a.batch; b0 += 64) all += __builtin_amdgcn_readlane(scan_over_wave(parts_of(b0 + lane), lane), 63);
-  const int number = paged_spread(w, all * a.kv_head);
-  if (number >= all * a.kv_head || (a.target && number >= a.slots)) return r;
-  int before = 0;
-  for (int b0 = 0; b0 < a.batch; b0 += 64) {
-    const int mine = parts_of(b0 + lane), upto = before + scan_over_wave(mine, lane);
-    const unsigned long long past = __builtin_amdgcn_ballot_w64(upto * a.kv_head > number);
-    if (past) {
-      const int l = __builtin_ctzll(past);
-      const int of_head = __builtin_amdgcn_readlane(mine, l), base = (__builtin_amdgcn_readlane(upto, l) - of_head) * a.kv_head;
-      r.b = b0 + l;
-      const Sequence s = sequence(a, r.b);
-      r.s.first = __builtin_amdgcn_readfirstlane(s.first);
-      r.s.n = __builtin_amdgcn_readfirstlane(s.n);
-      r.s.keys = __builtin_amdgcn_readfirstlane(s.keys);
-      r.s.past = __builtin_amdgcn_readfirstlane(s.past);
-      r.parts = paged_parts(paged_tiles(r.s.keys), per);
-      const int local = number - base;
-      r.head = __builtin_amdgcn_readfirstlane(local / of_head);
-      const int in_head = local - r.head * of_head;
-      r.block = __builtin_amdgcn_readfirstlane(in_head / r.parts);
-      r.p = in_head - r.block * r.parts;
-      r.number = number;
-      return r;
-    }
-    before = __builtin_amdgcn_readlane(upto, 63);
+struct Walk {
+  long x, end, length;  // position, end and length of the stretch
+  long upto;            // the line up to the end of the lane's sequence
+  int stretch, b0;      // b0: the first of the 64 sequences
+  Sequence mine;
+  __device__ __forceinline__ static PagedLine line(const PagedArgs& a, int n, int keys) {
+    const int rows_of_block = B::rows_of_block(n * a.group);
+    return a.shared ? paged_line(keys, n, a.group, a.causal ? a.step[B::many(n * a.group)] : 0, rows_of_block)
+                    : paged_line_of_ones(n, a.group, rows_of_block);
   }
-  return r;
-}
+  __device__ __forceinline__ void load(const PagedArgs& a, int from, long before, int lane) {
+    b0 = from;
+    mine = sequence(a, min(b0 + lane, a.batch - 1));
+    upto = before + scan_over_wave(b0 + lane < a.batch ? line(a, mine.n, mine.keys).all() * a.kv_head : 0);
+  }
+  // Makes out the stretch of work group w; false if there is none.
+  __device__ __forceinline__ bool begin(const PagedArgs& a, int w, int lane) {
+    load(a, 0, 0, lane);
+    long all = of_lane(upto, 63);
+    if (a.batch > 64) {
+      long more = 0;
+      for (int b = 64 + lane; b < a.batch; b += 64) {
+        const Sequence s = sequence(a, b);
+        more += line(a, s.n, s.keys).all() * a.kv_head;
+      }
+      all += of_lane(scan_over_wave(more), 63);
+    }
+    length = a.shared ? paged_stretch(all) : 1;
+    stretch = paged_spread(w, a.shared ? paged_stretches(all, length) : (int)all);
+    x = stretch * length;
+    end = min(x + length, all);
+    return x < all;
+  }
+  __device__ __forceinline__ bool next(const PagedArgs& a, int lane, Part& r) {
+    if (x >= end) return false;
+    unsigned long long past;
+    while (!(past = __builtin_amdgcn_ballot_w64(upto > x))) {
+      if (b0 + 64 >= a.batch) return false;
+      load(a, b0 + 64, of_lane(upto, 63), lane);
+    }
+    const int l = __builtin_ctzll(past);
+    r.b = b0 + l;
+    r.s.first = __builtin_amdgcn_readlane(mine.first, l);
+    r.s.n = __builtin_amdgcn_readlane(mine.n, l);
+    r.s.keys = __builtin_amdgcn_readlane(mine.keys, l);
+    r.s.past = __builtin_amdgcn_readlane(mine.past, l);
+    const PagedLine heads = line(a, r.s.n, r.s.keys);
+    const long of_head = heads.all(), base = of_lane(upto, l) - of_head * a.kv_head;
+    r.head = __builtin_amdgcn_readfirstlane(paged_divide(x - base, of_head));
+    const long from = base + r.head * of_head;
+    r.block = heads.blocks == 1 ? 0 : __builtin_amdgcn_readfirstlane(paged_block_at(heads, x - from));
+    const long item = from + heads.before(r.block), weight = heads.of(r.block);
+    const int rows = r.s.n * a.group, last = min(rows, (r.block + 1) * B::rows_of_block(rows)) - 1;
+    const int tiles = paged_tiles(paged_visible(r.s.keys, r.s.n, last / a.group, a.causal));
+    r.t0 = __builtin_amdgcn_readfirstlane(paged_tile_at(tiles, x - item, weight));
+    r.t1 = __builtin_amdgcn_readfirstlane(paged_tile_at(tiles, end - item, weight));
+    r.opens = item >= x;
+    r.whole = r.opens && item + weight <= end;
+    r.parts = r.whole || !r.opens ? 1 : __builtin_amdgcn_readfirstlane(paged_divide(item + weight - 1, length)) - stretch + 1;
+    r.place = paged_place(stretch, r.opens ? 0 : 1) - (r.opens ? 0 : 2);
+    r.stretch = stretch;
+    x = item + weight;
+    return true;
+  }
+};
 
 template <bool BF>
 __device__ __forceinline__ f4v mma16(h8 x, h8 y, f4v z) {
@@ -256,13 +285,10 @@ __device__ __forceinline__ void few_rows(const PagedArgs& a, const Part& w, char
 
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int m = lane & 15, g = lane >> 4;
-  const int rows = w.s.n * a.group, row0 = w.block * kRows;
-  const int last_token = (min(rows, row0 + kRows) - 1) / a.group;
-  const int seen = paged_visible(w.s.keys, w.s.n, last_token, a.causal);
+  const int rows = w.s.n * a.group, row0 = w.block * kRows, t0 = w.t0;
+  const int seen = paged_visible(w.s.keys, w.s.n, (min(rows, row0 + kRows) - 1) / a.group, a.causal);
   const int all_see = paged_visible(w.s.keys, w.s.n, row0 / a.group, a.causal);
-  int t0, t1;
-  paged_part(paged_tiles(seen), w.parts, w.p, t0, t1);
-  const int units = min(2 * t1, (seen + kUnit - 1) / kUnit) - 2 * t0;  // of the part
+  const int units = min(2 * w.t1, (seen + kUnit - 1) / kUnit) - 2 * t0;  // of the part
   const int u0 = 2 * t0 + max(units, 0) * wave / kFewWaves, u1 = 2 * t0 + max(units, 0) * (wave + 1) / kFewWaves;
 
   h8 qf[CB][kKS];
@@ -412,9 +438,9 @@ __device__ __forceinline__ void few_rows(const PagedArgs& a, const Part& w, char
     }
   }
 
-  if (a.target && w.p == 0 && threadIdx.x < kRows && row0 + (int)threadIdx.x < rows) {
+  if (a.shared && w.opens && threadIdx.x < kRows && row0 + (int)threadIdx.x < rows) {
     const int row = row0 + threadIdx.x, token = row / a.group, head = w.head * (int)a.group + row - token * (int)a.group;
-    a.places[(w.s.first + token) * a.head + head] = int2{w.number * slot_rows + (int)threadIdx.x, w.parts};
+    a.places[(w.s.first + token) * a.head + head] = int2{2 * w.stretch * slot_rows + (int)threadIdx.x, w.parts};
   }
   // the waves' sums, relative to the largest maximum
 #pragma unroll
@@ -449,12 +475,12 @@ __device__ __forceinline__ void few_rows(const PagedArgs& a, const Part& w, char
       sum += j.x == -INFINITY ? j.y : j.y * fast_exp2(j.x - mx);  // without keys 0, or NaN from a bad page
       x += *reinterpret_cast<const f4v*>(smem + v * G::kWaveBytes + row * G::kPitch + piece * 16);
     }
-    if (w.parts == 1) {
+    if (w.whole) {
       const int token = (row0 + row) / a.group, head = w.head * (int)a.group + (row0 + row - token * a.group);
       const float inv = sum == 0.f ? 0.f : 1.f / sum;
       store4<BF>(a.o + (((long)(w.s.first + token) * a.head + head) * D + piece * 4) * 2, x * inv);
     } else {
-      const long at = (long)w.number * slot_rows + row;
+      const long at = (long)w.place * slot_rows + row;
       *reinterpret_cast<f4v*>(a.part_o + at * D + piece * 4) = x;
       if (piece == 0) a.part_ml[at] = float2{mx, sum};
     }
@@ -506,9 +532,7 @@ __device__ __forceinline__ void many_rows(const PagedArgs& a, const Part& w, cha
     return t & 63;
   };
   const int rows = w.s.n * a.group, row0 = w.block * kManyRows, row0w = row0 + wave * kResident;
-  int t0, t1;
-  paged_part(paged_tiles(paged_visible(w.s.keys, w.s.n, (min(rows, row0 + kManyRows) - 1) / a.group, a.causal)), w.parts, w.p, t0, t1);
-  const int nt = t1 - t0;
+  const int t0 = w.t0, nt = w.t1 - t0;
   int ntw = 0, nfull = 0;  // tiles that the wave works on, those of them that all its rows see whole
   if (row0w < rows) {
     ntw = min(max(paged_tiles(paged_visible(w.s.keys, w.s.n, (min(rows, row0w + kResident) - 1) / a.group, a.causal)) - t0, 0), nt);
@@ -911,14 +935,14 @@ __device__ __forceinline__ void many_rows(const PagedArgs& a, const Part& w, cha
   const int lane = lane_now();
   float l_tot = l_run + other_half(l_run);
   if (bad_pages[0] | bad_pages[1] | bad_pages[2] | bad_pages[3]) l_tot = NAN;
-  const float f = w.parts > 1 ? 1.f : l_tot == 0.f ? 0.f : 1.f / l_tot;
+  const float f = !w.whole ? 1.f : l_tot == 0.f ? 0.f : 1.f / l_tot;
   char* const stage = smem + wave * (kResident * M::kPitch);
-  const long slot0 = (long)w.number * kManyRows + wave * kResident;
-  if (z.target && w.p == 0 && lane < kResident && row0w + lane < rows) {
+  const long slot0 = (long)w.place * kManyRows + wave * kResident;
+  if (z.shared && w.opens && lane < kResident && row0w + lane < rows) {
     const int row = row0w + lane, token = row / z.group, head = w.head * (int)z.group + row - token * (int)z.group;
-    z.places[(w.s.first + token) * z.head + head] = int2{(int)slot0 + lane, w.parts};
+    z.places[(w.s.first + token) * z.head + head] = int2{2 * w.stretch * kManyRows + wave * kResident + lane, w.parts};
   }
-  if (w.parts > 1 && lane < kResident && row0w + lane < rows) z.part_ml[slot0 + lane] = float2{mc, l_tot};
+  if (!w.whole && lane < kResident && row0w + lane < rows) z.part_ml[slot0 + lane] = float2{mc, l_tot};
 #pragma unroll
   for (int half = 0; half < D / 64; ++half) {
 #pragma unroll
@@ -937,7 +961,7 @@ __device__ __forceinline__ void many_rows(const PagedArgs& a, const Part& w, cha
       const int r = 4 * pass + (lane >> 4), row = row0w + r, piece = lane & 15;
       const f4v x = *reinterpret_cast<const f4v*>(stage + r * M::kPitch + piece * 16);
       if (row < rows) {
-        if (w.parts > 1) {
+        if (!w.whole) {
           *reinterpret_cast<f4v*>(z.part_o + (slot0 + r) * D + half * 64 + piece * 4) = x;
         } else {
           const int token = row / z.group, head = w.head * (int)z.group + row - token * (int)z.group;
@@ -954,23 +978,32 @@ __device__ __forceinline__ void many_rows(const PagedArgs& a, const Part& w, cha
 // A work group's part, by whichever of the two ways its sequence goes.
 // ---------------------------------------------------------------------------
 template <int D, int FEW, bool MANY, bool BF, bool Q8>
-__global__ void __launch_bounds__(kPagedThreads, 2) paged_forward_kernel(PagedArgs a) {
+__global__ void __launch_bounds__(kPagedThreads, 2) paged_forward_kernel(PagedArgs args) {
   using B = Blocks<FEW, MANY>;
   constexpr int kFewBytes = FEW ? kFewWaves * (FewGeom<D, FEW ? FEW / 16 : 1>::kWaveBytes + FEW * (int)sizeof(float2)) : 0;
   constexpr int kManyBytes = MANY ? ManyGeom<D, Q8>::kBytes : 0;
   __shared__ __attribute__((aligned(1024))) char smem[kFewBytes > kManyBytes ? kFewBytes : kManyBytes];
+  const PagedArgs& a = args;
   if (a.zero_rest) {
     const int rest = min(max(a.ends[a.batch - 1], 0), a.tokens);
     const long from = (long)rest * a.head * D * 2, to = (long)a.tokens * a.head * D * 2;
     for (long i = from + ((long)blockIdx.x * blockDim.x + threadIdx.x) * 16; i < to; i += (long)gridDim.x * blockDim.x * 16)
       *reinterpret_cast<u4v*>(a.o + i) = u4v{0, 0, 0, 0};
   }
-  const Part w = part_of<B>(a, blockIdx.x, threadIdx.x & 63);
-  if (w.b < 0) return;
-  if constexpr (MANY) {
-    if (B::many(w.s.n * a.group)) return many_rows<D, BF, Q8>(a, w, smem);
+  const int lane = threadIdx.x & 63;
+  Walk<B> walk;
+  if (!walk.begin(a, blockIdx.x, lane)) return;
+  for (;;) {
+    const PagedArgs a = args_again();
+    Part w;
+    if (!walk.next(a, lane, w)) return;
+    if (MANY && B::many(w.s.n * a.group)) {
+      if constexpr (MANY) many_rows<D, BF, Q8>(a, w, smem);
+    } else {
+      if constexpr (FEW != 0) few_rows<D, FEW / 16, BF, Q8>(a, w, smem, B::kMost);
+    }
+    __syncthreads();  // the next item takes the same LDS
   }
-  if constexpr (FEW != 0) few_rows<D, FEW / 16, BF, Q8>(a, w, smem, B::kMost);
 }
 
 // ---------------------------------------------------------------------------
@@ -996,7 +1029,7 @@ __device__ __forceinline__ Joined join_parts(const PagedArgs& a, int at, int par
     f4v x[kJoinAhead];
 #pragma unroll
     for (int u = 0; u < kJoinAhead; ++u) {
-      const long row = at + (long)min(p + u * step, parts - 1) * slot_rows;
+      const long row = at + (long)paged_place(0, min(p + u * step, parts - 1)) * slot_rows;
       ml[u] = a.part_ml[row];
       x[u] = *reinterpret_cast<const f4v*>(a.part_o + row * D + piece * 4);
     }
@@ -1018,7 +1051,7 @@ __global__ void __launch_bounds__(256) paged_join_kernel(PagedArgs a, int slot_r
   constexpr int kPieces = D / 4, kSlices = 256 / kPieces;
   __shared__ Joined sums[kSlices][kPieces];
   const int slice = threadIdx.x / kPieces, piece = threadIdx.x % kPieces, rows = a.tokens * a.head;
-  const int room = a.slots * slot_rows;
+  const long room = 2l * kPagedGroups * slot_rows;
   auto place = [&](int row) __attribute__((always_inline)) {
     if (row >= rows) return int2{0, 1};
     if (a.ends) {
@@ -1027,7 +1060,7 @@ __global__ void __launch_bounds__(256) paged_join_kernel(PagedArgs a, int slot_r
     }
     int2 r = a.places[row];
     // of tokens that ranges which make no sense left out it says anything
-    if (r.x < 0 || r.y < 1 || r.x >= room || r.y > (room - 1 - r.x) / slot_rows + 1) r.y = 1;
+    if (r.x < 0 || r.y < 1 || r.x + (2l * r.y + 1) * slot_rows > room) r.y = 1;
     return r;
   };
   auto store = [&](int row, const Joined& r) __attribute__((always_inline)) {
@@ -1237,17 +1270,13 @@ int check_cache(const paged_mha_cache* c, const paged_mha_batch* b) {
 
 long all_tokens(const paged_mha_batch* b) { return b->cu_seqlens ? b->tokens : (long)b->tokens * b->batch; }
 
-// Parts that a launch aims at, and the least tiles of one.
-constexpr int kTarget = 512, kLeast = 4;
-
 struct Launch {
-  int few;    // rows of a block of few, 0: there is none
-  bool many;  // whether there are blocks of kManyRows
+  int few;     // rows of a block of few, 0: there is none
+  bool many;   // whether there are blocks of kManyRows
   long items;  // at most
-  int target;
-  int slot_rows() const { return many ? kManyRows : few; }
-  long slots() const { return target ? items + target : 0; }
-  long grid() const { return (items + target + 7) / 8 * 8; }
+  bool shared;
+  int place_rows() const { return many ? kManyRows : few; }
+  long grid() const { return shared ? kPagedGroups : (items + 7) / 8 * 8; }
 };
 // The bits below which all offsets of 16 positions are 0, and whether the bits above fit 32.
 bool fits(const paged_mha_cache* c, const paged_mha_strides& s, int bytes, int& shift) {
@@ -1269,20 +1298,20 @@ Launch plan(const paged_mha_cache* c, const paged_mha_batch* b, int head, int ma
   const int least_rows = p.few ? p.few : kManyRows;
   const long blocks = b->cu_seqlens ? b->tokens * group / least_rows + b->batch : b->batch * ((b->tokens * group + least_rows - 1) / least_rows);
   p.items = blocks * c->kv_head;
-  p.target = (long)b->table_width * c->page_size > kLeast * kPagedTile ? kTarget : 0;
+  p.shared = (long)b->table_width * c->page_size * 4 > kPagedLeast;
   return p;
 }
 // Sums of the parts' rows, their maxima and totals, where each row of o has its parts.
 size_t workspace_bytes_of(const Launch& p, int d, long rows) {
-  return p.target ? (size_t)p.slots() * p.slot_rows() * (d * 4 + 8) + (size_t)rows * 8 : 0;
+  return p.shared ? (size_t)2 * kPagedGroups * p.place_rows() * (d * 4 + 8) + (size_t)rows * 8 : 0;
 }
 
 template <int D, int FEW, bool MANY, bool BF, bool Q8>
 int launch_forward(const Launch& p, const PagedArgs& a, hipStream_t stream) {
   if (launch(paged_forward_kernel<D, FEW, MANY, BF, Q8>, dim3(p.grid()), kPagedThreads, stream, a) != hipSuccess) return FUSED_MHA_ERR_LAUNCH;
-  if (!p.target) return FUSED_MHA_OK;
+  if (!p.shared) return FUSED_MHA_OK;
   const int rows = a.tokens * a.head, rows_of_group = MANY ? 256 / (D / 4) : 1;
-  return launch(paged_join_kernel<D, BF>, dim3((rows + rows_of_group - 1) / rows_of_group), 256, stream, a, p.slot_rows(), rows_of_group) == hipSuccess
+  return launch(paged_join_kernel<D, BF>, dim3((rows + rows_of_group - 1) / rows_of_group), 256, stream, a, p.place_rows(), rows_of_group) == hipSuccess
              ? FUSED_MHA_OK : FUSED_MHA_ERR_LAUNCH;
 }
 
@@ -1359,7 +1388,9 @@ static int check_forward(const paged_mha_cache* c, const paged_mha_batch* b, int
   if (head % c->kv_head) return PAGED_MHA_ERR_BAD_GROUP;
   if (head > (1 << 16) || all_tokens(b) * head >= (1L << 30)) return FUSED_MHA_ERR_TOO_LARGE;
   const Launch p = plan(c, b, head, max_new);
-  return p.grid() >= (1L << 30) || p.slots() * p.slot_rows() >= (1L << 30) ? FUSED_MHA_ERR_TOO_LARGE : FUSED_MHA_OK;
+  // the line's length fits 62 bits: an item weighs up to four for each key and new token
+  const double weight = 4. * ((double)b->table_width * c->page_size + kPagedOverhead + b->tokens);
+  return p.items >= (1L << 30) || p.items * weight >= 0x1p61 ? FUSED_MHA_ERR_TOO_LARGE : FUSED_MHA_OK;
 }
 
 size_t paged_mha_forward_workspace_bytes(const paged_mha_cache* c, const paged_mha_batch* b, int head, int max_new) {
@@ -1384,8 +1415,8 @@ int paged_mha_forward(const paged_mha_cache* c, const paged_mha_batch* b, const 
   a.k_scale = (const unsigned char*)c->key_scale, a.v_scale = (const unsigned char*)c->value_scale;
   a.table = b->page_table, a.keys = b->cache_seqlens, a.ends = b->cu_seqlens ? b->cu_seqlens + 1 : nullptr;
   a.part_o = (float*)workspace;
-  a.part_ml = (float2*)((char*)workspace + (size_t)p.slots() * p.slot_rows() * c->d * 4);
-  a.places = (int2*)(a.part_ml + (size_t)p.slots() * p.slot_rows());
+  a.part_ml = (float2*)((char*)workspace + (size_t)2 * kPagedGroups * p.place_rows() * c->d * 4);
+  a.places = (int2*)(a.part_ml + (size_t)2 * kPagedGroups * p.place_rows());
   a.ks = in_bytes(c->key_strides, bytes), a.vs = in_bytes(c->value_strides, bytes);
   a.kss = in_bytes(c->key_scale_strides, 1), a.vss = in_bytes(c->value_scale_strides, 1);
   a.q_batch = a.ends ? 0 : q_st->batch * 2, a.q_seq = q_st->seq * 2, a.q_head = q_st->head * 2;
@@ -1395,7 +1426,8 @@ int paged_mha_forward(const paged_mha_cache* c, const paged_mha_batch* b, const 
   a.group = FmhaDivisor(head / c->kv_head), a.page_size = FmhaDivisor(c->page_size);
   a.c = scale * kLog2e;
   a.causal = causal != 0, a.zero_rest = zero_rest != 0 && a.ends;
-  a.target = p.target, a.least = kLeast, a.slots = (int)p.slots();
+  a.shared = p.shared;
+  a.step[0] = paged_step(p.few, head / c->kv_head), a.step[1] = paged_step(kManyRows, head / c->kv_head);
   if (p.many) fits(c, c->key_strides, bytes, a.k_shift), fits(c, c->value_strides, bytes, a.v_shift);
   return with_types(c, [&](auto d, auto bf, auto q8) {
     constexpr int D = decltype(d)::value;

@@ -5,29 +5,16 @@
 #include "block_map.h"
 
 // Rows of a sequence and key head: its new tokens times the query heads of the key head, token by token.  A block is a number
-// of neighbouring rows, an item a block of one sequence and key head, a part some of the key tiles of an item: the unit of
-// work of a work group.  All items of a sequence have the same number of parts, numbered key head by key head, block by block.
+// of neighbouring rows, an item a block of one sequence and key head with the tiles of keys that it sees.  Items stand in a
+// line, sequence by sequence, key head by key head, block by block, each as long as its work (its weight), and each work group
+// gets a stretch of the line of the same length: the end of an item that begins in an earlier stretch, whole items, and the
+// beginning of one that goes on in the next.  An item that lies in several stretches is joined afterwards, part by part.
+// All work groups have the same amount of work whatever the lengths are, and none needs to know what others do.
 constexpr int kPagedTile = 64;  // keys
 
 FMHA_HOST_DEVICE int paged_tiles(int keys) { return (keys + kPagedTile - 1) / kPagedTile; }
 
 FMHA_HOST_DEVICE int paged_blocks(int rows, int rows_of_block) { return (rows + rows_of_block - 1) / rows_of_block; }
-
-// Tiles of a part, of so many in all that there are about `target` parts, but none of fewer than `least` tiles.
-FMHA_HOST_DEVICE int paged_tiles_of_part(long tiles, int target, int least) {
-  const long even = (tiles + target - 1) / target;
-  return even > least ? (int)even : least;
-}
-
-// Parts of an item of so many tiles: at least one, which writes the result of items without keys.
-FMHA_HOST_DEVICE int paged_parts(int tiles, int tiles_of_part) { return tiles <= tiles_of_part ? 1 : (tiles + tiles_of_part - 1) / tiles_of_part; }
-
-// Tiles first .. end-1 of part p; none where there are fewer tiles than parts.
-FMHA_HOST_DEVICE void paged_part(int tiles, int parts, int p, int& first, int& end) {
-  const int each = tiles / parts, more = tiles - each * parts;
-  first = p * each + (p < more ? p : more);
-  end = first + each + (p < more ? 1 : 0);
-}
 
 // Keys that the last of new tokens 0 .. i sees.
 FMHA_HOST_DEVICE int paged_visible(int keys, int new_tokens, int i, bool causal) {
@@ -35,11 +22,78 @@ FMHA_HOST_DEVICE int paged_visible(int keys, int new_tokens, int i, bool causal)
   return seen < 0 ? 0 : seen;
 }
 
-// Work group w of a launch takes part paged_spread(w, parts), if that is one: neighbouring parts, which read the same keys, go to the
-// same XCD (work groups go round-robin over the 8).  The launch has at least 8 * ceil(parts / 8) work groups.
-FMHA_HOST_DEVICE int paged_spread(int w, int parts) {
-  const int run = (parts + 7) >> 3;
-  return (w >> 3) < run ? (w & 7) * run + (w >> 3) : parts;
+// Weights of the items of a sequence and key head, in quarters of a key: of block k `first + step * (k + 1)`, about the keys that
+// the block sees and something for its beginning and end.
+constexpr int kPagedOverhead = 64;  // keys
+struct PagedLine {
+  long first;
+  int step, blocks;
+  FMHA_HOST_DEVICE long before(int k) const { return k * first + (long)step * k * (k + 1) / 2; }
+  FMHA_HOST_DEVICE long of(int k) const { return first + (long)step * (k + 1); }
+  FMHA_HOST_DEVICE long all() const { return before(blocks); }
+};
+// step: 0 without a causal mask, else paged_step, which divides.
+FMHA_HOST_DEVICE int paged_step(int rows_of_block, int group) { return 4 * rows_of_block / group; }
+template <typename Int>  // int or FmhaDivisor
+FMHA_HOST_DEVICE PagedLine paged_line(int keys, int new_tokens, const Int& group, int step, int rows_of_block) {
+  const int hidden = step == 0 ? 0 : new_tokens < keys ? new_tokens : keys;
+  return PagedLine{4 * (long)(keys - hidden + kPagedOverhead), step, paged_blocks(new_tokens * group, rows_of_block)};
 }
+// Items that count one each, for launches with a work group for every item.
+template <typename Int>
+FMHA_HOST_DEVICE PagedLine paged_line_of_ones(int new_tokens, const Int& group, int rows_of_block) {
+  return PagedLine{1, 0, paged_blocks(new_tokens * group, rows_of_block)};
+}
+
+// n / d where that is below 2^20: by floats, put right.
+FMHA_HOST_DEVICE int paged_divide(long n, long d) {
+  int q = (int)((float)n / (float)d);
+  if (q * d > n) --q;
+  if ((q + 1) * d <= n) ++q;
+  return q;
+}
+
+// Length of a stretch: the same for up to kPagedGroups of them, which is as many work groups as the device runs at a time, but
+// not so short that a work group has little else to do than to begin and end.
+constexpr int kPagedGroupsLog = 9, kPagedGroups = 1 << kPagedGroupsLog;
+constexpr int kPagedLeastLog = 10, kPagedLeast = 1 << kPagedLeastLog;  // 256 keys
+FMHA_HOST_DEVICE long paged_stretch(long all) {
+  const long even = (all + kPagedGroups - 1) >> kPagedGroupsLog;
+  return even > kPagedLeast ? even : kPagedLeast;
+}
+// How many there are, or a few more.
+FMHA_HOST_DEVICE int paged_stretches(long all, long length) {
+  return length > kPagedLeast ? kPagedGroups : (int)((all + kPagedLeast - 1) >> kPagedLeastLog);
+}
+
+// Block in which position x (from 0 to all() - 1) of a key head's line lies.
+FMHA_HOST_DEVICE int paged_block_at(const PagedLine& line, long x) {
+  int lo = 0, hi = line.blocks - 1;
+  while (lo < hi) {
+    const int mid = (lo + hi + 1) / 2;
+    if (line.before(mid) <= x) lo = mid;
+    else hi = mid - 1;
+  }
+  return lo;
+}
+
+// The tile at which a stretch that begins or ends `into` an item of that weight begins or ends.
+FMHA_HOST_DEVICE int paged_tile_at(int tiles, long into, long weight) {
+  if (into <= 0) return 0;
+  if (into >= weight) return tiles;
+  const int at = (int)((float)into * ((float)tiles / (float)weight));  // grows with `into`, the same on both sides
+  return at < tiles ? at : tiles;
+}
+
+// Work group w of a launch has stretch paged_spread(w, stretches), if that is one: neighbouring stretches, which read the same keys,
+// go to the same XCD (work groups go round-robin over the 8).  The launch has at least 8 * ceil(stretches / 8) work groups.
+FMHA_HOST_DEVICE int paged_spread(int w, int stretches) {
+  const int run = (stretches + 7) >> 3;
+  return (w >> 3) < run ? (w & 7) * run + (w >> 3) : stretches;
+}
+
+// Where parts of an item that begins in stretch r lie: stretch s has two places, 2 s for the end of an item and 2 s + 1 for the
+// beginning of one.  An item that is all of a stretch and more, begun before, is an end.
+FMHA_HOST_DEVICE int paged_place(int r, int part) { return 2 * (r + part) + (part == 0 ? 1 : 0); }
 
 #endif  // PAGED_PLAN_H_

@@ -259,37 +259,92 @@ def host_program(tmp_path, body):
     return subprocess.run([str(exe)], stdout=subprocess.PIPE).stdout.decode()
 
 
-def test_parts_cover_every_tile_once(tmp_path):
+def test_stretches_cover_every_tile_once(tmp_path):
+    """Random batches: the items of all stretches, found one after the other as the kernel finds them, are each there whole; parts
+    have places of their own, which are those that the item's first part says; stretches differ by no more than an item's rounding."""
     out = host_program(tmp_path, r"""
+#include <map>
+struct Seq { int n, keys; };
 int main() {
-  for (int tiles = 0; tiles < 300; ++tiles)
-    for (int per = 1; per < 40; ++per) {
-      const int parts = paged_parts(tiles, per);
-      if (parts < 1 || (long)parts * per < tiles) return puts("too few"), 1;
-      for (int fewer = tiles; fewer >= 0; fewer -= 7) {  // an item whose rows see less than the sequence has
-        int at = 0;
-        for (int p = 0; p < parts; ++p) {
-          int first, end;
-          paged_part(fewer, parts, p, first, end);
-          if (first != at || end < first || end - first > per) return puts("gap"), 1;
-          at = end;
+  unsigned seed = 1;
+  auto rnd = [&](int n) { seed = seed * 1664525u + 1013904223u; return (int)((seed >> 8) % (unsigned)n); };
+  for (int round = 0; round < 3000; ++round) {
+    const int batch = 1 + rnd(12), kv = 1 + rnd(4), group = 1 + rnd(9), rows_of_block = rnd(2) ? 32 : 128;
+    const bool causal = rnd(2), ones = rnd(8) == 0;
+    std::vector<Seq> seqs(batch);
+    std::vector<PagedLine> lines(batch);
+    long all = 0;
+    for (int b = 0; b < batch; ++b) {
+      seqs[b] = {rnd(3) ? rnd(3) : rnd(300), rnd(3) ? rnd(500) : rnd(20000)};
+      lines[b] = ones ? paged_line_of_ones(seqs[b].n, group, rows_of_block) : paged_line(seqs[b].keys, seqs[b].n, group, causal ? paged_step(rows_of_block, group) : 0, rows_of_block);
+      all += lines[b].all() * kv;
+    }
+    const long length = ones ? 1 : paged_stretch(all);
+    const int stretches = ones ? (int)all : paged_stretches(all, length);
+    if (stretches * length < all || (!ones && stretches > kPagedGroups)) return puts("stretches"), 1;
+    struct Item { int next = 0, tiles = -1, parts = 0, told = 0, first = 0; };
+    std::map<std::vector<int>, Item> items;
+    std::map<int, int> places;
+    for (int s = 0; s < stretches; ++s) {
+      long x = s * length;
+      const long end = x + length < all ? x + length : all;
+      while (x < end) {
+        long before = 0;
+        int b = 0;
+        while (before + lines[b].all() * kv <= x) before += lines[b++].all() * kv;
+        const int head = paged_divide(x - before, lines[b].all());
+        const long from = before + head * lines[b].all();
+        const int block = paged_block_at(lines[b], x - from);
+        const long item = from + lines[b].before(block), weight = lines[b].of(block);
+        if (weight <= 0 || item > x || item + weight <= x) return puts("block"), 1;
+        const int rows = seqs[b].n * group, last = (rows < (block + 1) * rows_of_block ? rows : (block + 1) * rows_of_block) - 1;
+        const int tiles = paged_tiles(paged_visible(seqs[b].keys, seqs[b].n, last / group, causal));
+        const int t0 = paged_tile_at(tiles, x - item, weight), t1 = paged_tile_at(tiles, end - item, weight);
+        const bool opens = item >= x, whole = opens && item + weight <= end;
+        Item& it = items[{b, head, block}];
+        if (opens != (it.parts == 0) || t0 != it.next || t1 < t0) return puts("gap"), 1;
+        if (opens) {
+          it.told = whole ? 1 : paged_divide(item + weight - 1, length) - s + 1;
+          it.first = s;
         }
-        if (at != fewer) return puts("end"), 1;
+        if (!whole) {
+          const int place = paged_place(s, opens ? 0 : 1) - (opens ? 0 : 2);
+          if (place < 0 || place >= 2 * stretches || places[place]++) return puts("place"), 1;
+          if (place != paged_place(it.first, it.parts)) return puts("place of the part"), 1;
+        }
+        it.next = t1, it.tiles = tiles, ++it.parts;
+        x = item + weight;
       }
     }
-  for (long tiles = 0; tiles < 5000; tiles += 3)
-    for (int target : {1, 7, 512})
-      for (int least : {1, 4}) {
-        const int per = paged_tiles_of_part(tiles, target, least);
-        if (per < least || (long)per * target < tiles) return puts("target"), 1;
-      }
+    for (int b = 0; b < batch; ++b)
+      for (int h = 0; h < kv; ++h)
+        for (int k = 0; k < lines[b].blocks; ++k) {
+          const Item it = items[{b, h, k}];
+          if (it.next != it.tiles || it.parts != it.told || (ones && it.parts != 1)) return puts("not whole"), 1;
+        }
+  }
   puts("ok");
 }
 """)
     assert out == "ok\n"
 
 
-def test_work_groups_take_every_part_once(tmp_path):
+def test_division(tmp_path):
+    out = host_program(tmp_path, r"""
+int main() {
+  unsigned long seed = 1;
+  auto rnd = [&](int bits) { seed = seed * 6364136223846793005ul + 1442695040888963407ul; return (long)(seed >> (64 - bits)); };
+  for (int i = 0; i < 4000000; ++i) {
+    const long d = rnd(1 + i % 41) + 1, n = d * rnd(1 + i % 20) + rnd(1 + i % 41) % d;
+    if (paged_divide(n, d) != n / d || paged_divide(n / d * d, d) != n / d) return puts("wrong"), 1;
+  }
+  puts("ok");
+}
+""")
+    assert out == "ok\n"
+
+
+def test_work_groups_take_every_stretch_once(tmp_path):
     out = host_program(tmp_path, r"""
 int main() {
   for (int parts = 0; parts < 3000; ++parts) {
@@ -301,31 +356,6 @@ int main() {
     }
     for (int p = 0; p < parts; ++p)
       if (taken[p] != 1) return puts("not once"), 1;
-  }
-  puts("ok");
-}
-""")
-    assert out == "ok\n"
-
-
-def test_there_is_room_for_every_part(tmp_path):
-    """As many slots and work groups as a launch has are enough for the parts of any lengths: at most `target` and one for each item."""
-    out = host_program(tmp_path, r"""
-int main() {
-  unsigned seed = 1;
-  auto rnd = [&](int n) { seed = seed * 1664525u + 1013904223u; return (int)((seed >> 8) % (unsigned)n); };
-  for (int n = 0; n < 20000; ++n) {
-    const int batch = 1 + rnd(40), kv = 1 + rnd(8), target = 512, least = 4;
-    std::vector<int> blocks(batch), tiles(batch);
-    long all = 0, items = 0;
-    for (int b = 0; b < batch; ++b) {
-      blocks[b] = rnd(4), tiles[b] = rnd(rnd(4) ? 60 : 3000);
-      all += (long)blocks[b] * tiles[b] * kv, items += (long)blocks[b] * kv;
-    }
-    const int per = paged_tiles_of_part(all, target, least);
-    long parts = 0;
-    for (int b = 0; b < batch; ++b) parts += (long)blocks[b] * kv * paged_parts(tiles[b], per);
-    if (parts > items + target) return puts("too many"), 1;
   }
   puts("ok");
 }
