@@ -132,7 +132,10 @@ struct Blocks {
   static constexpr int kMost = MANY ? kManyRows : FEW;  // rows of a slot
   static __device__ __forceinline__ bool many(int rows) { return MANY && (FEW == 0 || rows > kFewRows); }
   static __device__ __forceinline__ int rows_of_block(int rows) { return many(rows) ? kManyRows : FEW; }
-  static __device__ __forceinline__ int count(int rows) { return paged_blocks(rows, rows_of_block(rows)); }
+  // What an item costs beside its keys, in keys, and what a second item in a stretch does, in quarters of a key: about two tiles of
+  // 64 where a block has many rows, one where it has few.
+  static __device__ __forceinline__ int overhead(int rows) { return many(rows) ? 128 : 64; }
+  static constexpr int kSecond = MANY ? 2 * 4 * 64 : 4 * 64;
 };
 
 // What a work group does of an item.
@@ -152,31 +155,76 @@ struct Walk {
   long x, end, length;  // position, end and length of the stretch
   long upto;            // the line up to the end of the lane's sequence
   int stretch, b0;      // b0: the first of the 64 sequences
+  float per_length;     // not 0: items have whole stretches, as many as paged_parts says
   Sequence mine;
-  __device__ __forceinline__ static PagedLine line(const PagedArgs& a, int n, int keys) {
-    const int rows_of_block = B::rows_of_block(n * a.group);
-    return a.shared ? paged_line(keys, n, a.group, a.causal ? a.step[B::many(n * a.group)] : 0, rows_of_block)
-                    : paged_line_of_ones(n, a.group, rows_of_block);
+  __device__ __forceinline__ static PagedLine weights(const PagedArgs& a, int n, int keys) {
+    const int rows = n * a.group;
+    return paged_line(keys, n, a.group, a.causal ? a.step[B::many(rows)] : 0, B::rows_of_block(rows), B::overhead(rows));
+  }
+  __device__ __forceinline__ PagedLine line(const PagedArgs& a, int n, int keys) const {
+    if (a.shared && per_length == 0.f) return weights(a, n, keys);
+    return paged_line_of_parts(a.shared ? paged_parts(heaviest(a, n, keys), per_length) : 1, n, a.group, B::rows_of_block(n * a.group));
+  }
+  __device__ __forceinline__ static float heaviest(const PagedArgs& a, int n, int keys) {
+    return (float)(4 * (keys + B::overhead(n * a.group)));
   }
   __device__ __forceinline__ void load(const PagedArgs& a, int from, long before, int lane) {
     b0 = from;
     mine = sequence(a, min(b0 + lane, a.batch - 1));
+    scan(a, before, lane);
+  }
+  __device__ __forceinline__ void scan(const PagedArgs& a, long before, int lane) {
     upto = before + scan_over_wave(b0 + lane < a.batch ? line(a, mine.n, mine.keys).all() * a.kv_head : 0);
   }
   // Makes out the stretch of work group w; false if there is none.
+  //
+  // A stretch that ends where an item does costs one beginning less, so if there is a length for which all items have whole
+  // stretches, no more than kPagedGroups together, that is not longer by more than that, it is taken: of 64 lengths, from the even
+  // one up to three times that, by as many lanes.
   __device__ __forceinline__ bool begin(const PagedArgs& a, int w, int lane) {
+    per_length = 0.f;
     load(a, 0, 0, lane);
     long all = of_lane(upto, 63);
-    if (a.batch > 64) {
+    if (!a.shared) {
+      if (a.batch > 64) {
+        long more = 0;
+        for (int b = 64 + lane; b < a.batch; b += 64) {
+          const Sequence s = sequence(a, b);
+          more += line(a, s.n, s.keys).all() * a.kv_head;
+        }
+        all += of_lane(scan_over_wave(more), 63);
+      }
+      length = 1;
+      stretch = paged_spread(w, (int)all);
+    } else if (a.batch > 64) {
       long more = 0;
       for (int b = 64 + lane; b < a.batch; b += 64) {
         const Sequence s = sequence(a, b);
-        more += line(a, s.n, s.keys).all() * a.kv_head;
+        more += weights(a, s.n, s.keys).all() * a.kv_head;
       }
       all += of_lane(scan_over_wave(more), 63);
+      length = paged_stretch(all);
+      stretch = paged_spread(w, paged_stretches(all, length));
+    } else {
+      length = paged_stretch(all);
+      const float mine_in = 1.f / ((float)length * (1.f + lane * (1.f / 32.f)));
+      const float weight = heaviest(a, mine.n, mine.keys);
+      const int items = paged_blocks(mine.n * a.group, B::rows_of_block(mine.n * a.group)) * a.kv_head;
+      int parts = 0;
+      for (int b = 0; b < a.batch; ++b)
+        parts += __builtin_amdgcn_readlane(items, b) * paged_parts(__uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(weight), b)), mine_in);
+      const unsigned long long fit = __builtin_amdgcn_ballot_w64(parts <= kPagedGroups && (float)length * (lane * (1.f / 32.f)) <= B::kSecond);
+      if (fit) {
+        const int l = __builtin_ctzll(fit);
+        per_length = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(mine_in), l));
+        all = __builtin_amdgcn_readlane(parts, l);
+        length = 1;
+        scan(a, 0, lane);
+        stretch = paged_spread(w, (int)all);
+      } else {
+        stretch = paged_spread(w, paged_stretches(all, length));
+      }
     }
-    length = a.shared ? paged_stretch(all) : 1;
-    stretch = paged_spread(w, a.shared ? paged_stretches(all, length) : (int)all);
     x = stretch * length;
     end = min(x + length, all);
     return x < all;
@@ -1389,7 +1437,7 @@ static int check_forward(const paged_mha_cache* c, const paged_mha_batch* b, int
   if (head > (1 << 16) || all_tokens(b) * head >= (1L << 30)) return FUSED_MHA_ERR_TOO_LARGE;
   const Launch p = plan(c, b, head, max_new);
   // the line's length fits 62 bits: an item weighs up to four for each key and new token
-  const double weight = 4. * ((double)b->table_width * c->page_size + kPagedOverhead + b->tokens);
+  const double weight = 4. * ((double)b->table_width * c->page_size + 128 + b->tokens);
   return p.items >= (1L << 30) || p.items * weight >= 0x1p61 ? FUSED_MHA_ERR_TOO_LARGE : FUSED_MHA_OK;
 }
 

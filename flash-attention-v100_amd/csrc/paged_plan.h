@@ -22,9 +22,7 @@ FMHA_HOST_DEVICE int paged_visible(int keys, int new_tokens, int i, bool causal)
   return seen < 0 ? 0 : seen;
 }
 
-// Weights of the items of a sequence and key head, in quarters of a key: of block k `first + step * (k + 1)`, about the keys that
-// the block sees and something for its beginning and end.
-constexpr int kPagedOverhead = 64;  // keys
+// Weights of the items of a sequence and key head: of block k `first + step * (k + 1)`.
 struct PagedLine {
   long first;
   int step, blocks;
@@ -32,18 +30,21 @@ struct PagedLine {
   FMHA_HOST_DEVICE long of(int k) const { return first + (long)step * (k + 1); }
   FMHA_HOST_DEVICE long all() const { return before(blocks); }
 };
-// step: 0 without a causal mask, else paged_step, which divides.
+// In quarters of a key: about the keys that a block sees, and something for its beginning and end.  step: 0 without a causal mask,
+// else paged_step, which divides.
 FMHA_HOST_DEVICE int paged_step(int rows_of_block, int group) { return 4 * rows_of_block / group; }
 template <typename Int>  // int or FmhaDivisor
-FMHA_HOST_DEVICE PagedLine paged_line(int keys, int new_tokens, const Int& group, int step, int rows_of_block) {
+FMHA_HOST_DEVICE PagedLine paged_line(int keys, int new_tokens, const Int& group, int step, int rows_of_block, int overhead) {
   const int hidden = step == 0 ? 0 : new_tokens < keys ? new_tokens : keys;
-  return PagedLine{4 * (long)(keys - hidden + kPagedOverhead), step, paged_blocks(new_tokens * group, rows_of_block)};
+  return PagedLine{4 * (long)(keys - hidden + overhead), step, paged_blocks(new_tokens * group, rows_of_block)};
 }
-// Items that count one each, for launches with a work group for every item.
+// In stretches, where every item has a whole number of them.
 template <typename Int>
-FMHA_HOST_DEVICE PagedLine paged_line_of_ones(int new_tokens, const Int& group, int rows_of_block) {
-  return PagedLine{1, 0, paged_blocks(new_tokens * group, rows_of_block)};
+FMHA_HOST_DEVICE PagedLine paged_line_of_parts(int parts, int new_tokens, const Int& group, int rows_of_block) {
+  return PagedLine{parts, 0, paged_blocks(new_tokens * group, rows_of_block)};
 }
+// Parts of an item of that weight, none of them longer than 1 / per_length.
+FMHA_HOST_DEVICE int paged_parts(float weight, float per_length) { return (int)(weight * per_length) + 1; }
 
 // n / d where that is below 2^20: by floats, put right.
 FMHA_HOST_DEVICE int paged_divide(long n, long d) {

@@ -276,7 +276,7 @@ int main() {
     long all = 0;
     for (int b = 0; b < batch; ++b) {
       seqs[b] = {rnd(3) ? rnd(3) : rnd(300), rnd(3) ? rnd(500) : rnd(20000)};
-      lines[b] = ones ? paged_line_of_ones(seqs[b].n, group, rows_of_block) : paged_line(seqs[b].keys, seqs[b].n, group, causal ? paged_step(rows_of_block, group) : 0, rows_of_block);
+      lines[b] = ones ? paged_line_of_parts(1 + rnd(5), seqs[b].n, group, rows_of_block) : paged_line(seqs[b].keys, seqs[b].n, group, causal ? paged_step(rows_of_block, group) : 0, rows_of_block, 64);
       all += lines[b].all() * kv;
     }
     const long length = ones ? 1 : paged_stretch(all);
@@ -320,7 +320,7 @@ int main() {
       for (int h = 0; h < kv; ++h)
         for (int k = 0; k < lines[b].blocks; ++k) {
           const Item it = items[{b, h, k}];
-          if (it.next != it.tiles || it.parts != it.told || (ones && it.parts != 1)) return puts("not whole"), 1;
+          if (it.next != it.tiles || it.parts != it.told || (ones && it.parts != lines[b].first)) return puts("not whole"), 1;
         }
   }
   puts("ok");
