@@ -45,6 +45,11 @@ struct PagedArgs {
   int k_shift, v_shift;  // offsets of 16 positions in the cache are multiples of 2^shift bytes, fewer than 2^32
 };
 
+// Says that a pointer is to global memory, which the compiler knows of a kernel's parameters alone: without it loads are flat ones,
+// for which every wait for LDS waits too.
+template <typename T>
+__device__ __forceinline__ void in_global(T*& p) { p = (T*)(__attribute__((address_space(1))) T*)(uintptr_t)p; }
+
 // The kernel's arguments as they lie in memory, asked for where they are needed again: kept in registers across a main loop they
 // are spilled.
 __device__ __forceinline__ PagedArgs args_again() {
@@ -56,7 +61,10 @@ __device__ __forceinline__ PagedArgs args_again() {
   } words;
 #pragma unroll
   for (unsigned i = 0; i < sizeof(PagedArgs) / 4; ++i) words.w[i] = from[i];
-  return __builtin_bit_cast(PagedArgs, words);
+  PagedArgs a = __builtin_bit_cast(PagedArgs, words);
+  in_global(a.q), in_global(a.k), in_global(a.v), in_global(a.k_scale), in_global(a.v_scale), in_global(a.o), in_global(a.table);
+  in_global(a.keys), in_global(a.ends), in_global(a.part_o), in_global(a.part_ml), in_global(a.places);
+  return a;
 }
 
 struct Sequence {
@@ -368,9 +376,12 @@ __device__ __forceinline__ void few_rows(const PagedArgs& a, const Part& w, char
     bad |= __builtin_amdgcn_ballot_w64(none && stretch0 + lane < 2 * u1) != 0;
     if (none) ids = 0;
   };
-  u4v kr[2][kLoads], vr[2][kLoads];
-  unsigned ksc[2], vsc[2];
-  auto load = [&](int u) __attribute__((always_inline)) {
+  constexpr int kDepth = Q8 ? 2 : 1;  // units on their way
+  struct Unit {
+    u4v k[2][kLoads], v[2][kLoads];
+    unsigned k_sc[2], v_sc[2];
+  } ahead[kDepth];
+  auto load = [&](int u, Unit& x) __attribute__((always_inline)) {
     if (2 * u - ids0 >= 64) fetch_ids(2 * u);
 #pragma unroll
     for (int R = 0; R < 2; ++R) {
@@ -381,16 +392,16 @@ __device__ __forceinline__ void few_rows(const PagedArgs& a, const Part& w, char
       const char* const kb = k_head + id * a.ks.page + (long)slot * a.ks.slot;
       const char* const vb = v_head + id * a.vs.page + (long)slot * a.vs.slot;
 #pragma unroll
-      for (int i = 0; i < kLoads; ++i) kr[R][i] = *reinterpret_cast<const u4v*>(kb + (unsigned)(r * a.ks.slot + col + 64 * i));
+      for (int i = 0; i < kLoads; ++i) x.k[R][i] = *reinterpret_cast<const u4v*>(kb + (unsigned)(r * a.ks.slot + col + 64 * i));
 #pragma unroll
-      for (int i = 0; i < kLoads; ++i) vr[R][i] = *reinterpret_cast<const u4v*>(vb + (unsigned)(r * a.vs.slot + col + 64 * i));
+      for (int i = 0; i < kLoads; ++i) x.v[R][i] = *reinterpret_cast<const u4v*>(vb + (unsigned)(r * a.vs.slot + col + 64 * i));
       if constexpr (Q8) {
-        ksc[R] = a.k_scale[id * a.kss.page + (long)(slot + r) * a.kss.slot + (long)w.head * a.kss.head];
-        vsc[R] = a.v_scale[id * a.vss.page + (long)(slot + r) * a.vss.slot + (long)w.head * a.vss.head];
+        x.k_sc[R] = a.k_scale[id * a.kss.page + (long)(slot + r) * a.kss.slot + (long)w.head * a.kss.head];
+        x.v_sc[R] = a.v_scale[id * a.vss.page + (long)(slot + r) * a.vss.slot + (long)w.head * a.vss.head];
       }
     }
   };
-  auto to_lds = [&]() __attribute__((always_inline)) {
+  auto to_lds = [&](const Unit& x) __attribute__((always_inline)) {
 #pragma unroll
     for (int R = 0; R < 2; ++R) {
 #pragma unroll
@@ -400,12 +411,12 @@ __device__ __forceinline__ void few_rows(const PagedArgs& a, const Part& w, char
 #pragma unroll
           for (int e = 0; e < 2; ++e) {
             const int chunk = ((2 * (q4 & 1) + e) ^ swz(r16 >> 2)) * 16;
-            *reinterpret_cast<u4v*>(k_tile + at + chunk) = from_e4m3<BF>(kr[R][i][2 * e], kr[R][i][2 * e + 1], scale_of(ksc[R]));
-            *reinterpret_cast<u4v*>(v_tile + at + chunk) = from_e4m3<BF>(vr[R][i][2 * e], vr[R][i][2 * e + 1], scale_of(vsc[R]));
+            *reinterpret_cast<u4v*>(k_tile + at + chunk) = from_e4m3<BF>(x.k[R][i][2 * e], x.k[R][i][2 * e + 1], scale_of(x.k_sc[R]));
+            *reinterpret_cast<u4v*>(v_tile + at + chunk) = from_e4m3<BF>(x.v[R][i][2 * e], x.v[R][i][2 * e + 1], scale_of(x.v_sc[R]));
           }
         } else {
-          *reinterpret_cast<u4v*>(k_tile + T::block_off(R, i) + lane * 16) = kr[R][i];
-          *reinterpret_cast<u4v*>(v_tile + T::block_off(R, i) + lane * 16) = vr[R][i];
+          *reinterpret_cast<u4v*>(k_tile + T::block_off(R, i) + lane * 16) = x.k[R][i];
+          *reinterpret_cast<u4v*>(v_tile + T::block_off(R, i) + lane * 16) = x.v[R][i];
         }
       }
     }
@@ -422,13 +433,13 @@ __device__ __forceinline__ void few_rows(const PagedArgs& a, const Part& w, char
   const unsigned ka0 = opaque_lds_address(k_tile + rows16_off<D>(lane, 0)), ka1 = opaque_lds_address(k_tile + rows16_off<D>(lane, 1));
   const Cols16<D> va(v_tile, lane);
 
-  if (u0 < u1) {
-    fetch_ids(2 * u0);
-    load(u0);
-  }
-  for (int u = u0; u < u1; ++u) {
-    to_lds();
-    if (u + 1 < u1) load(u + 1);
+  if (u0 < u1) fetch_ids(2 * u0);
+#pragma unroll
+  for (int n = 0; n < kDepth; ++n)
+    if (u0 + n < u1) load(u0 + n, ahead[n]);
+  auto unit = [&](int u, Unit& x) __attribute__((always_inline)) {
+    to_lds(x);
+    if (u + kDepth < u1) load(u + kDepth, x);
     f4v s[CB][2];
 #pragma unroll
     for (int kk = 0; kk < kKS; ++kk) {
@@ -445,18 +456,18 @@ __device__ __forceinline__ void few_rows(const PagedArgs& a, const Part& w, char
     bool moved = false;
 #pragma unroll
     for (int cb = 0; cb < CB; ++cb) {
-      float x[8];
+      float p[8];
 #pragma unroll
-      for (int e = 0; e < 8; ++e) x[e] = s[cb][e >> 2][e & 3] * a.c;
+      for (int e = 0; e < 8; ++e) p[e] = s[cb][e >> 2][e & 3] * a.c;
       if (key0 + kUnit > all_see) {
         const int left = sees[cb] - key0 - 16 * (g >> 1) - 4 * (g & 1);
 #pragma unroll
         for (int e = 0; e < 8; ++e)
-          if (8 * (e >> 2) + (e & 3) >= left) x[e] = -INFINITY;
+          if (8 * (e >> 2) + (e & 3) >= left) p[e] = -INFINITY;
       }
-      float mx = x[0];
+      float mx = p[0];
 #pragma unroll
-      for (int e = 1; e < 8; ++e) mx = fmaxf(mx, x[e]);
+      for (int e = 1; e < 8; ++e) mx = fmaxf(mx, p[e]);
       mx = fmaxf(max_over_groups(mx), mc[cb]);
       const float from = mx == -INFINITY ? 0.f : mx;  // no key yet: every exponential is 0
       alpha[cb] = fast_exp2(mc[cb] - from);
@@ -465,12 +476,12 @@ __device__ __forceinline__ void few_rows(const PagedArgs& a, const Part& w, char
       float sum = 0.f;
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
-        x[e] = fast_exp2(x[e] - from);
-        sum += x[e];
+        p[e] = fast_exp2(p[e] - from);
+        sum += p[e];
       }
       l[cb] = l[cb] * alpha[cb] + sum;
 #pragma unroll
-      for (int e = 0; e < 4; ++e) pf[cb][e] = pack2<BF>(x[2 * e], x[2 * e + 1]);
+      for (int e = 0; e < 4; ++e) pf[cb][e] = pack2<BF>(p[2 * e], p[2 * e + 1]);
     }
     if (__builtin_amdgcn_ballot_w64(moved)) {
 #pragma unroll
@@ -484,6 +495,11 @@ __device__ __forceinline__ void few_rows(const PagedArgs& a, const Part& w, char
 #pragma unroll
       for (int cb = 0; cb < CB; ++cb) o[cb][db] = mma16<BF>(vf, __builtin_bit_cast(h8, pf[cb]), o[cb][db]);
     }
+  };
+  for (int u = u0; u < u1; u += kDepth) {
+#pragma unroll
+    for (int n = 0; n < kDepth; ++n)
+      if (u + n < u1) unit(u + n, ahead[n]);
   }
 
   if (a.shared && w.opens && threadIdx.x < kRows && row0 + (int)threadIdx.x < rows) {
