@@ -315,26 +315,47 @@ __device__ __forceinline__ float over_groups_sum(float x) {
 
 // ---------------------------------------------------------------------------
 // Attention, blocks of 16 * CB rows.  Work group = 4 waves that share the rows and split the part's keys: units of 32 keys,
-// neighbouring ones to a wave, no barrier between them.  A unit comes to registers while the one before is worked on, goes to the
-// wave's own tile of LDS (converted there from 8 bits), scores are formed transposed, S^T[keys][rows], so that the 16-bit
-// probabilities are the second product's operand as they are (Geom16).  At the end the waves' sums are joined in LDS.
+// neighbouring ones to a wave, no barrier between them, a tile of LDS for each wave.  Scores are formed transposed,
+// S^T[keys][rows], so that the 16-bit probabilities are the second product's operand as they are (Geom16).  At the end the waves'
+// sums are joined in LDS.
+//
+// 16-bit cache: a unit comes to registers while the one before is worked on, then goes to the tile.
+// 8-bit cache: units are copied to LDS as they are, two at a time, and converted where they become operands.  Keys' scales go into
+// the conversion.  Values' scales, which differ along the second product's sum, go into the probabilities: exp2(t + e - m') with
+// the value's exponent e and a maximum m' of its own of t + e, so that what counts most is 1 whatever the scales are.
 // ---------------------------------------------------------------------------
 constexpr int kPagedThreads = 256;
 constexpr int kFewWaves = kPagedThreads / 64;
 constexpr int kUnit = 32;
-template <int D, int CB>
+template <int D, int CB, bool Q8>
 struct FewGeom {
   static constexpr int kRows = 16 * CB;
-  static constexpr int kTileBytes = kUnit * D * 2;
+  static constexpr int kTileBytes = kUnit * D * (Q8 ? 1 : 2);                 // of keys or values
+  static constexpr int kSlotBytes = 2 * kTileBytes + (Q8 ? 2 * kUnit * 4 : 0);  // and their scales
+  static constexpr int kSlots = Q8 ? 2 : 1;
   static constexpr int kPitch = D * 4 + 16;  // of a row of sums in LDS
   static constexpr int kJoinBytes = kRows * kPitch;
-  static constexpr int kWaveBytes = (2 * kTileBytes > kJoinBytes ? 2 * kTileBytes : kJoinBytes + 1023) / 1024 * 1024;
+  static constexpr int kWaveBytes = ((kSlots * kSlotBytes > kJoinBytes ? kSlots * kSlotBytes : kJoinBytes) + 1023) / 1024 * 1024;
 };
+
+// A byte for each lane to the lane's dword from `lds` on, past the compiler's wait counts like copy16.
+__device__ __forceinline__ void copy_byte(const unsigned char* from, unsigned lds) {
+  unsigned saved_m0;
+  asm volatile(
+      "s_mov_b32 %0, m0\n\t"
+      "s_mov_b32 m0, %2\n\t"
+      "s_nop 0\n\t"
+      "global_load_lds_ubyte %1, off\n\t"
+      "s_mov_b32 m0, %0"
+      : "=&s"(saved_m0)
+      : "v"(from), "s"(lds)
+      : "memory");
+}
 
 template <int D, int CB, bool BF, bool Q8>
 __device__ __forceinline__ void few_rows(const PagedArgs& a, const Part& w, char* smem, int slot_rows) {
   using T = SwzTile<D>;
-  using G = FewGeom<D, CB>;
+  using G = FewGeom<D, CB, Q8>;
   constexpr int kRows = G::kRows, kNC = T::kNC, kKS = D / 32, kDB = D / 16;
   constexpr int kLoads = Q8 ? kNC / 2 : kNC;  // of 16 positions: 64 bytes of each
   float2(*const join)[kRows] = reinterpret_cast<float2(*)[kRows]>(smem + kFewWaves * G::kWaveBytes);
@@ -347,6 +368,29 @@ __device__ __forceinline__ void few_rows(const PagedArgs& a, const Part& w, char
   const int units = min(2 * w.t1, (seen + kUnit - 1) / kUnit) - 2 * t0;  // of the part
   const int u0 = 2 * t0 + max(units, 0) * wave / kFewWaves, u1 = 2 * t0 + max(units, 0) * (wave + 1) / kFewWaves;
 
+  // page numbers of 64 stretches of 16 positions, from stretch ids0 on
+  bool bad = w.s.past;
+  int ids = 0, ids0 = 0;
+  auto fetch_ids = [&](int stretch0) __attribute__((always_inline)) {
+    ids0 = stretch0;
+    const int at = min((stretch0 + lane) * 16, w.s.keys - 1);
+    ids = a.table[w.b * a.table_stride + at / a.page_size];
+    const bool none = (unsigned)ids >= (unsigned)a.pages;
+    // of stretches that are behind the wave's last one nothing is said
+    bad |= __builtin_amdgcn_ballot_w64(none && stretch0 + lane < 2 * u1) != 0;
+    if (none) ids = 0;
+  };
+  if (u0 < u1) fetch_ids(2 * u0);
+  // Positions 16 R .. of unit u: their page, the first's slot, and how many there are less one.  Those past the last key are it again.
+  struct Stretch {
+    long id;
+    int slot, last;
+  };
+  auto stretch_of = [&](int u, int R) __attribute__((always_inline)) {
+    const int stretch = min(2 * u + R, (w.s.keys - 1) >> 4), pos = stretch * 16, page_at = pos / a.page_size;
+    return Stretch{__builtin_amdgcn_readlane(ids, stretch - ids0), pos - page_at * (int)a.page_size, w.s.keys - 1 - pos};
+  };
+
   h8 qf[CB][kKS];
   int sees[CB];  // keys that the lane's row of a column block sees
 #pragma unroll
@@ -358,148 +402,226 @@ __device__ __forceinline__ void few_rows(const PagedArgs& a, const Part& w, char
     for (int kk = 0; kk < kKS; ++kk) qf[cb][kk] = *reinterpret_cast<const h8*>(at + kk * 64 + g * 16);
   }
 
-  char* const k_tile = smem + wave * G::kWaveBytes;
-  char* const v_tile = k_tile + G::kTileBytes;
+  char* const tile = smem + wave * G::kWaveBytes;
   const int r16 = lane >> 2, q4 = lane & 3;
   const char* const k_head = a.k + (long)w.head * a.ks.head;
   const char* const v_head = a.v + (long)w.head * a.vs.head;
-  const int col = Q8 ? q4 * 16 : (q4 ^ swz(r16 >> 2)) * 16;
-  bool bad = w.s.past;
-  // page numbers of 64 stretches of 16 positions, from stretch ids0 on
-  int ids = 0, ids0 = 0;
-  auto fetch_ids = [&](int stretch0) __attribute__((always_inline)) {
-    ids0 = stretch0;
-    const int at = min((stretch0 + lane) * 16, w.s.keys - 1);
-    ids = a.table[w.b * a.table_stride + at / a.page_size];
-    const bool none = (unsigned)ids >= (unsigned)a.pages;
-    // of stretches that are behind the wave's last one nothing is said
-    bad |= __builtin_amdgcn_ballot_w64(none && stretch0 + lane < 2 * u1) != 0;
-    if (none) ids = 0;
-  };
-  constexpr int kDepth = Q8 ? 2 : 1;  // units on their way
-  struct Unit {
-    u4v k[2][kLoads], v[2][kLoads];
-    unsigned k_sc[2], v_sc[2];
-  } ahead[kDepth];
-  auto load = [&](int u, Unit& x) __attribute__((always_inline)) {
-    if (2 * u - ids0 >= 64) fetch_ids(2 * u);
-#pragma unroll
-    for (int R = 0; R < 2; ++R) {
-      const int stretch = min(2 * u + R, (w.s.keys - 1) >> 4);  // positions past the last one: the last one again
-      const int pos = stretch * 16, page_at = pos / a.page_size, slot = pos - page_at * a.page_size;
-      const long id = __builtin_amdgcn_readlane(ids, stretch - ids0);
-      const int r = min(r16, w.s.keys - 1 - pos);
-      const char* const kb = k_head + id * a.ks.page + (long)slot * a.ks.slot;
-      const char* const vb = v_head + id * a.vs.page + (long)slot * a.vs.slot;
-#pragma unroll
-      for (int i = 0; i < kLoads; ++i) x.k[R][i] = *reinterpret_cast<const u4v*>(kb + (unsigned)(r * a.ks.slot + col + 64 * i));
-#pragma unroll
-      for (int i = 0; i < kLoads; ++i) x.v[R][i] = *reinterpret_cast<const u4v*>(vb + (unsigned)(r * a.vs.slot + col + 64 * i));
-      if constexpr (Q8) {
-        x.k_sc[R] = a.k_scale[id * a.kss.page + (long)(slot + r) * a.kss.slot + (long)w.head * a.kss.head];
-        x.v_sc[R] = a.v_scale[id * a.vss.page + (long)(slot + r) * a.vss.slot + (long)w.head * a.vss.head];
-      }
-    }
-  };
-  auto to_lds = [&](const Unit& x) __attribute__((always_inline)) {
-#pragma unroll
-    for (int R = 0; R < 2; ++R) {
-#pragma unroll
-      for (int i = 0; i < kLoads; ++i) {
-        if constexpr (Q8) {
-          const int at = T::block_off(R, 2 * i + (q4 >> 1)) + r16 * 64;
-#pragma unroll
-          for (int e = 0; e < 2; ++e) {
-            const int chunk = ((2 * (q4 & 1) + e) ^ swz(r16 >> 2)) * 16;
-            *reinterpret_cast<u4v*>(k_tile + at + chunk) = from_e4m3<BF>(x.k[R][i][2 * e], x.k[R][i][2 * e + 1], scale_of(x.k_sc[R]));
-            *reinterpret_cast<u4v*>(v_tile + at + chunk) = from_e4m3<BF>(x.v[R][i][2 * e], x.v[R][i][2 * e + 1], scale_of(x.v_sc[R]));
-          }
-        } else {
-          *reinterpret_cast<u4v*>(k_tile + T::block_off(R, i) + lane * 16) = x.k[R][i];
-          *reinterpret_cast<u4v*>(v_tile + T::block_off(R, i) + lane * 16) = x.v[R][i];
-        }
-      }
-    }
-  };
 
   f4v o[CB][kDB];
-  float mc[CB], l[CB];
+  float mc[CB], l[CB], mv[CB];  // mv: m' of an 8-bit cache
 #pragma unroll
   for (int cb = 0; cb < CB; ++cb) {
-    mc[cb] = -INFINITY, l[cb] = 0.f;
+    mc[cb] = mv[cb] = -INFINITY, l[cb] = 0.f;
 #pragma unroll
     for (int db = 0; db < kDB; ++db) o[cb][db] = f4v{0.f, 0.f, 0.f, 0.f};
   }
-  const unsigned ka0 = opaque_lds_address(k_tile + rows16_off<D>(lane, 0)), ka1 = opaque_lds_address(k_tile + rows16_off<D>(lane, 1));
-  const Cols16<D> va(v_tile, lane);
-
-  if (u0 < u1) fetch_ids(2 * u0);
+  // exponents of the lane's 8 keys: scores times c, without those that its row does not see
+  auto exponents = [&](int u, int cb, const f4v (&s)[2], float (&t)[8]) __attribute__((always_inline)) {
 #pragma unroll
-  for (int n = 0; n < kDepth; ++n)
-    if (u0 + n < u1) load(u0 + n, ahead[n]);
-  auto unit = [&](int u, Unit& x) __attribute__((always_inline)) {
-    to_lds(x);
-    if (u + kDepth < u1) load(u + kDepth, x);
-    f4v s[CB][2];
+    for (int e = 0; e < 8; ++e) t[e] = s[e >> 2][e & 3] * a.c;
+    if (u * kUnit + kUnit > all_see) {
+      const int left = sees[cb] - u * kUnit - 16 * (g >> 1) - 4 * (g & 1);
 #pragma unroll
-    for (int kk = 0; kk < kKS; ++kk) {
-#pragma unroll
-      for (int p = 0; p < 2; ++p) {
-        const h8 kf = rows16_at<D>(ka0, ka1, p, kk);
-#pragma unroll
-        for (int cb = 0; cb < CB; ++cb) s[cb][p] = mma16<BF>(kf, qf[cb][kk], kk == 0 ? f4v{0.f, 0.f, 0.f, 0.f} : s[cb][p]);
-      }
-    }
-    const int key0 = u * kUnit;
-    u4v pf[CB];
-    float alpha[CB];
-    bool moved = false;
-#pragma unroll
-    for (int cb = 0; cb < CB; ++cb) {
-      float p[8];
-#pragma unroll
-      for (int e = 0; e < 8; ++e) p[e] = s[cb][e >> 2][e & 3] * a.c;
-      if (key0 + kUnit > all_see) {
-        const int left = sees[cb] - key0 - 16 * (g >> 1) - 4 * (g & 1);
-#pragma unroll
-        for (int e = 0; e < 8; ++e)
-          if (8 * (e >> 2) + (e & 3) >= left) p[e] = -INFINITY;
-      }
-      float mx = p[0];
-#pragma unroll
-      for (int e = 1; e < 8; ++e) mx = fmaxf(mx, p[e]);
-      mx = fmaxf(max_over_groups(mx), mc[cb]);
-      const float from = mx == -INFINITY ? 0.f : mx;  // no key yet: every exponential is 0
-      alpha[cb] = fast_exp2(mc[cb] - from);
-      moved |= mx != mc[cb];
-      mc[cb] = mx;
-      float sum = 0.f;
-#pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        p[e] = fast_exp2(p[e] - from);
-        sum += p[e];
-      }
-      l[cb] = l[cb] * alpha[cb] + sum;
-#pragma unroll
-      for (int e = 0; e < 4; ++e) pf[cb][e] = pack2<BF>(p[2 * e], p[2 * e + 1]);
-    }
-    if (__builtin_amdgcn_ballot_w64(moved)) {
-#pragma unroll
-      for (int cb = 0; cb < CB; ++cb)
-#pragma unroll
-        for (int db = 0; db < kDB; ++db) o[cb][db] *= alpha[cb];
-    }
-#pragma unroll
-    for (int db = 0; db < kDB; ++db) {
-      const h8 vf = va.at(0, 0, db);
-#pragma unroll
-      for (int cb = 0; cb < CB; ++cb) o[cb][db] = mma16<BF>(vf, __builtin_bit_cast(h8, pf[cb]), o[cb][db]);
+      for (int e = 0; e < 8; ++e)
+        if (8 * (e >> 2) + (e & 3) >= left) t[e] = -INFINITY;
     }
   };
-  for (int u = u0; u < u1; u += kDepth) {
+  // the maximum of theirs and all lanes' of the row and m; no key yet is taken as 0: every exponential is 0 then
+  auto raise = [&](const float (&t)[8], float& m, float& from) __attribute__((always_inline)) {
+    float mx = t[0];
 #pragma unroll
-    for (int n = 0; n < kDepth; ++n)
-      if (u + n < u1) unit(u + n, ahead[n]);
+    for (int e = 1; e < 8; ++e) mx = fmaxf(mx, t[e]);
+    mx = fmaxf(max_over_groups(mx), m);
+    from = mx == -INFINITY ? 0.f : mx;
+    const float alpha = fast_exp2(m - from);
+    m = mx;
+    return alpha;
+  };
+
+  if constexpr (!Q8) {
+    const int col = (q4 ^ swz(r16 >> 2)) * 16;
+    char* const v_tile = tile + G::kTileBytes;
+    u4v kr[2][kLoads], vr[2][kLoads];
+    auto load = [&](int u) __attribute__((always_inline)) {
+      if (2 * u - ids0 >= 64) fetch_ids(2 * u);
+#pragma unroll
+      for (int R = 0; R < 2; ++R) {
+        const Stretch t = stretch_of(u, R);
+        const int r = min(r16, t.last);
+        const char* const kb = k_head + t.id * a.ks.page + (long)t.slot * a.ks.slot;
+        const char* const vb = v_head + t.id * a.vs.page + (long)t.slot * a.vs.slot;
+#pragma unroll
+        for (int i = 0; i < kLoads; ++i) kr[R][i] = *reinterpret_cast<const u4v*>(kb + (unsigned)(r * a.ks.slot + col + 64 * i));
+#pragma unroll
+        for (int i = 0; i < kLoads; ++i) vr[R][i] = *reinterpret_cast<const u4v*>(vb + (unsigned)(r * a.vs.slot + col + 64 * i));
+      }
+    };
+    const unsigned ka0 = opaque_lds_address(tile + rows16_off<D>(lane, 0)), ka1 = opaque_lds_address(tile + rows16_off<D>(lane, 1));
+    const Cols16<D> va(v_tile, lane);
+    if (u0 < u1) load(u0);
+    for (int u = u0; u < u1; ++u) {
+#pragma unroll
+      for (int R = 0; R < 2; ++R) {
+#pragma unroll
+        for (int i = 0; i < kLoads; ++i) {
+          *reinterpret_cast<u4v*>(tile + T::block_off(R, i) + lane * 16) = kr[R][i];
+          *reinterpret_cast<u4v*>(v_tile + T::block_off(R, i) + lane * 16) = vr[R][i];
+        }
+      }
+      if (u + 1 < u1) load(u + 1);
+      f4v s[CB][2];
+#pragma unroll
+      for (int kk = 0; kk < kKS; ++kk) {
+#pragma unroll
+        for (int p = 0; p < 2; ++p) {
+          const h8 kf = rows16_at<D>(ka0, ka1, p, kk);
+#pragma unroll
+          for (int cb = 0; cb < CB; ++cb) s[cb][p] = mma16<BF>(kf, qf[cb][kk], kk == 0 ? f4v{0.f, 0.f, 0.f, 0.f} : s[cb][p]);
+        }
+      }
+      u4v pf[CB];
+      float alpha[CB];
+      bool moved = false;
+#pragma unroll
+      for (int cb = 0; cb < CB; ++cb) {
+        float t[8], from, sum = 0.f;
+        exponents(u, cb, s[cb], t);
+        alpha[cb] = raise(t, mc[cb], from);
+        moved |= alpha[cb] != 1.f;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          t[e] = fast_exp2(t[e] - from);
+          sum += t[e];
+        }
+        l[cb] = l[cb] * alpha[cb] + sum;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) pf[cb][e] = pack2<BF>(t[2 * e], t[2 * e + 1]);
+      }
+      if (__builtin_amdgcn_ballot_w64(moved)) {
+#pragma unroll
+        for (int cb = 0; cb < CB; ++cb)
+#pragma unroll
+          for (int db = 0; db < kDB; ++db) o[cb][db] *= alpha[cb];
+      }
+#pragma unroll
+      for (int db = 0; db < kDB; ++db) {
+        const h8 vf = va.at(0, 0, db);
+#pragma unroll
+        for (int cb = 0; cb < CB; ++cb) o[cb][db] = mma16<BF>(vf, __builtin_bit_cast(h8, pf[cb]), o[cb][db]);
+      }
+    }
+  } else {
+    typedef __attribute__((address_space(3))) u2v lds_u2v;
+    typedef __attribute__((address_space(3))) u4v lds_u4v;
+    typedef __attribute__((address_space(3))) unsigned lds_u;
+    typedef int i2v __attribute__((ext_vector_type(2)));
+    typedef __attribute__((address_space(3))) i2v lds_i2v;
+    const unsigned lds0 = (unsigned)(uintptr_t)(__attribute__((address_space(3))) char*)tile;
+    // Chunk c of 16 bytes of row r16 of rows 16 R .. lies at (c ^ swz(r16 >> 2) ^ 2 R) * 16 of the row's 64 bytes, so that neither
+    // reads below meet in a bank.
+    const int col = (q4 ^ swz(r16 >> 2)) * 16;
+    constexpr int kBack = 960 * (kLoads - 1), kOps = 4 * kLoads + 1;  // see copy16_blocks; copies of a unit
+    auto copy = [&](const char* from, int off, unsigned to) __attribute__((always_inline)) {
+      if constexpr (kLoads == 1) copy16(wave_uniform(from), off, smem + __builtin_amdgcn_readfirstlane(to - lds0) + wave * G::kWaveBytes);
+      else copy16_blocks<kLoads>(wave_uniform(from - kBack), off + kBack, __builtin_amdgcn_readfirstlane(to));
+    };
+    auto ask = [&](int u, unsigned slot) __attribute__((always_inline)) {
+      if (2 * u - ids0 >= 64) fetch_ids(2 * u);
+      const Stretch t[2] = {stretch_of(u, 0), stretch_of(u, 1)};
+#pragma unroll
+      for (int R = 0; R < 2; ++R) {
+        const int r = min(r16, t[R].last), at = R * kLoads * 1024;
+        copy(k_head + t[R].id * a.ks.page + (long)t[R].slot * a.ks.slot, r * a.ks.slot + (col ^ (32 * R)), slot + at);
+        copy(v_head + t[R].id * a.vs.page + (long)t[R].slot * a.vs.slot, r * a.vs.slot + (col ^ (32 * R)), slot + G::kTileBytes + at);
+      }
+      // scales of the 32 keys, then of the values
+      const bool R = lane & 16;
+      const long id = R ? t[1].id : t[0].id, at = (R ? t[1].slot : t[0].slot) + min(lane & 15, R ? t[1].last : t[0].last);
+      const unsigned char* const ks = a.k_scale + (long)w.head * a.kss.head + id * a.kss.page + at * a.kss.slot;
+      const unsigned char* const vs = a.v_scale + (long)w.head * a.vss.head + id * a.vss.page + at * a.vss.slot;
+      copy_byte(lane < 32 ? ks : vs, __builtin_amdgcn_readfirstlane(slot + 2 * G::kTileBytes));
+    };
+    unsigned k_at[2];  // the lane's row of keys: 8 p + (m & 7) of rows 16 (m >> 3) ..
+    unsigned k_at_scale[2], v_at_scale[2];
+#pragma unroll
+    for (int p = 0; p < 2; ++p) {
+      const int R = m >> 3, row = 8 * p + (m & 7);
+      k_at[p] = lds0 + R * kLoads * 1024 + row * 64 + (((g >> 1) ^ swz(row >> 2) ^ (2 * R)) * 16) + (g & 1) * 8;
+      k_at_scale[p] = lds0 + 2 * G::kTileBytes + (16 * R + row) * 4;
+      v_at_scale[p] = lds0 + 2 * G::kTileBytes + (32 + 16 * (g >> 1) + 8 * p + 4 * (g & 1)) * 4;
+    }
+    unsigned v_at;  // of 8 keys of the lane's group, in the order of its probabilities, a pair of lanes has 16 features of each
+    {
+      const int R = g >> 1, row = 4 * (g & 1) + (m >> 1 & 3) + 8 * (m >> 3);
+      v_at = lds0 + G::kTileBytes + R * kLoads * 1024 + row * 64 + ((swz(row >> 2) ^ (2 * R)) * 16) + (m & 1) * 8;
+    }
+    if (u0 < u1) ask(u0, lds0);
+    if (u0 + 1 < u1) ask(u0 + 1, lds0 + G::kSlotBytes);
+    for (int u = u0; u < u1; ++u) {
+      const unsigned slot = (u - u0) & 1 ? G::kSlotBytes : 0;
+      if (u + 1 < u1) wait_vm<kOps>();
+      else wait_vm<0>();
+      asm volatile("" ::: "memory");
+      f4v s[CB][2];
+#pragma unroll
+      for (int p = 0; p < 2; ++p) {
+        const float scale = scale_of(*(const lds_u*)(uintptr_t)(k_at_scale[p] + slot));
+#pragma unroll
+        for (int kk = 0; kk < kKS; ++kk) {
+          const u2v x = *(const lds_u2v*)(uintptr_t)(((k_at[p] + slot) ^ (kk & 1) * 32) + (kk >> 1) * 1024);
+          const h8 kf = __builtin_bit_cast(h8, from_e4m3<BF>(x[0], x[1], scale));
+#pragma unroll
+          for (int cb = 0; cb < CB; ++cb) s[cb][p] = mma16<BF>(kf, qf[cb][kk], kk == 0 ? f4v{0.f, 0.f, 0.f, 0.f} : s[cb][p]);
+        }
+      }
+      float e8[8];  // exponents of the lane's values
+#pragma unroll
+      for (int p = 0; p < 2; ++p) {
+        const u4v x = *(const lds_u4v*)(uintptr_t)(v_at_scale[p] + slot);
+#pragma unroll
+        for (int r = 0; r < 4; ++r) e8[4 * p + r] = (float)(int)(x[r] - 127);
+      }
+      u4v pf[CB];
+      float alpha[CB];
+      bool moved = false;
+#pragma unroll
+      for (int cb = 0; cb < CB; ++cb) {
+        float t[8], from, sum = 0.f;
+        exponents(u, cb, s[cb], t);
+        const float less = raise(t, mc[cb], from);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) sum += fast_exp2(t[e] - from);
+        l[cb] = l[cb] * less + sum;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) t[e] += e8[e];
+        alpha[cb] = raise(t, mv[cb], from);
+        moved |= alpha[cb] != 1.f;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) pf[cb][e] = pack2<BF>(fast_exp2(t[2 * e] - from), fast_exp2(t[2 * e + 1] - from));
+      }
+      if (__builtin_amdgcn_ballot_w64(moved)) {
+#pragma unroll
+        for (int cb = 0; cb < CB; ++cb)
+#pragma unroll
+          for (int db = 0; db < kDB; ++db) o[cb][db] *= alpha[cb];
+      }
+#pragma unroll
+      for (int db = 0; db < kDB; ++db) {
+        const i2v x = __builtin_amdgcn_ds_read_tr8_b64_v2i32((lds_i2v*)(uintptr_t)(((v_at + slot) ^ (db & 3) * 16) + (db >> 2) * 1024));
+        const h8 vf = __builtin_bit_cast(h8, from_e4m3<BF>(x[0], x[1], 1.f));
+#pragma unroll
+        for (int cb = 0; cb < CB; ++cb) o[cb][db] = mma16<BF>(vf, __builtin_bit_cast(h8, pf[cb]), o[cb][db]);
+      }
+      staged_rows_read();  // the slot has been read
+      if (u + 2 < u1) ask(u + 2, lds0 + slot);
+    }
+    // to the scale of the sums: the exponents are at most the largest of the scales apart
+#pragma unroll
+    for (int cb = 0; cb < CB; ++cb) {
+      const float f = mc[cb] == -INFINITY ? 0.f : fast_exp2(mv[cb] - mc[cb]);
+#pragma unroll
+      for (int db = 0; db < kDB; ++db) o[cb][db] *= f;
+    }
   }
 
   if (a.shared && w.opens && threadIdx.x < kRows && row0 + (int)threadIdx.x < rows) {
@@ -1044,7 +1166,7 @@ __device__ __forceinline__ void many_rows(const PagedArgs& a, const Part& w, cha
 template <int D, int FEW, bool MANY, bool BF, bool Q8>
 __global__ void __launch_bounds__(kPagedThreads, 2) paged_forward_kernel(PagedArgs args) {
   using B = Blocks<FEW, MANY>;
-  constexpr int kFewBytes = FEW ? kFewWaves * (FewGeom<D, FEW ? FEW / 16 : 1>::kWaveBytes + FEW * (int)sizeof(float2)) : 0;
+  constexpr int kFewBytes = FEW ? kFewWaves * (FewGeom<D, FEW ? FEW / 16 : 1, Q8>::kWaveBytes + FEW * (int)sizeof(float2)) : 0;
   constexpr int kManyBytes = MANY ? ManyGeom<D, Q8>::kBytes : 0;
   __shared__ __attribute__((aligned(1024))) char smem[kFewBytes > kManyBytes ? kFewBytes : kManyBytes];
   const PagedArgs& a = args;
