@@ -36,8 +36,8 @@ struct PagedArgs {
   CacheStrides ks, vs, kss, vss;
   long q_batch, q_seq, q_head, table_stride;  // of q in bytes
   int batch, new_tokens, tokens;              // new_tokens: of each sequence, where ends is null; tokens: in all
-  int head, kv_head, pages, width;
-  FmhaDivisor group, page_size;  // group: query heads of a key head
+  int head, pages, width;
+  FmhaDivisor kv_head, group, page_size;  // group: query heads of a key head
   float c;                       // scale * log2(e)
   int causal, zero_rest;
   int shared;   // items are shared out (paged_plan.h), otherwise each has a work group
@@ -115,6 +115,11 @@ __device__ __forceinline__ long of_lane(long x, int lane) {
   const unsigned lo = __builtin_amdgcn_readlane((unsigned)x, lane), hi = __builtin_amdgcn_readlane((unsigned)((unsigned long)x >> 32), lane);
   return (long)(((unsigned long)hi << 32) | lo);
 }
+// Says that all lanes have the same value, which then takes a scalar register.
+__device__ __forceinline__ int same(int x) { return __builtin_amdgcn_readfirstlane(x); }
+__device__ __forceinline__ float same(float x) { return __int_as_float(same(__float_as_int(x))); }
+__device__ __forceinline__ long same(long x) { return of_lane(x, 0); }
+
 // The sum over lanes 0 .. the lane's own, by moves inside rows of 16 lanes and of the last lane of a row, or of two, to the next.
 template <int kMove, int kRows>
 __device__ __forceinline__ long moved(long x) {
@@ -140,12 +145,16 @@ struct Blocks {
   static constexpr int kMost = MANY ? kManyRows : FEW;  // rows of a slot
   static __device__ __forceinline__ bool many(int rows) { return MANY && (FEW == 0 || rows > kFewRows); }
   static __device__ __forceinline__ int rows_of_block(int rows) { return many(rows) ? kManyRows : FEW; }
-  // What an item costs beside its keys, in keys, and what a second item in a stretch does, in quarters of a key: about two tiles of
-  // 64 where a block has many rows, one where it has few.
-  static __device__ __forceinline__ int overhead(int rows) { return many(rows) ? 128 : 64; }
-  static constexpr int kSecond = MANY ? 2 * 4 * 64 : 4 * 64;
+  // What an item costs beside its keys, in keys: about three tiles where a block has many rows, one where it has few.
+  static __device__ __forceinline__ int overhead(int rows) { return many(rows) ? 192 : 64; }
+  // Weight of a key: 4 for a block of many rows while another shares its CU.  Beside such blocks those of few rows, which wait for
+  // memory, take half of it.
+  static __device__ __forceinline__ int of_key(int rows) { return MANY && FEW && !many(rows) ? 2 : 4; }
+  // A block of many rows alone on its CU takes 0.55 of the time.  What parts cost (256: a tile): an item more in a stretch, and of
+  // many rows to write their sums and to read them again, of up to two in each stretch or of one.
+  static constexpr float kAlone = MANY ? 0.55f : 1.f;
+  static constexpr float kStretchesCost = (MANY ? 3 + 14 : 1) * 256, kPartsCost = MANY ? 7 * 256 : 0;
 };
-
 // What a work group does of an item.
 struct Part {
   int b, head, block;
@@ -157,92 +166,115 @@ struct Part {
   Sequence s;
 };
 
-// The items of a work group's stretch, one after the other; all lanes together.  A lane has one of 64 sequences in its registers.
+__device__ __forceinline__ float max_over_wave(float x) {
+#pragma unroll
+  for (int d = 1; d < 16; d *= 2) x = fmaxf(x, __shfl_xor(x, d));
+  return max_over_groups(x);
+}
+
+// A work group's items, one after the other (ways to share them: paged_plan.h); all lanes together, each with one of 64 sequences
+// in its registers.
 template <typename B>
 struct Walk {
-  long x, end, length;  // position, end and length of the stretch
+  enum Way { kStretches, kParts, kWhole };
+  long x, end, length;  // position; end of the stretch and its length
   long upto;            // the line up to the end of the lane's sequence
   int stretch, b0;      // b0: the first of the 64 sequences
-  float per_length;     // not 0: items have whole stretches, as many as paged_parts says
+  int round, items;     // of kWhole
+  float per_length;     // of kParts: for paged_parts
+  Way way;
   Sequence mine;
   __device__ __forceinline__ static PagedLine weights(const PagedArgs& a, int n, int keys) {
     const int rows = n * a.group;
-    return paged_line(keys, n, a.group, a.causal ? a.step[B::many(rows)] : 0, B::rows_of_block(rows), B::overhead(rows));
-  }
-  __device__ __forceinline__ PagedLine line(const PagedArgs& a, int n, int keys) const {
-    if (a.shared && per_length == 0.f) return weights(a, n, keys);
-    return paged_line_of_parts(a.shared ? paged_parts(heaviest(a, n, keys), per_length) : 1, n, a.group, B::rows_of_block(n * a.group));
+    return paged_line(keys, n, a.group, a.causal ? a.step[B::many(rows)] : 0, B::rows_of_block(rows), B::overhead(rows), B::of_key(rows));
   }
   __device__ __forceinline__ static float heaviest(const PagedArgs& a, int n, int keys) {
-    return (float)(4 * (keys + B::overhead(n * a.group)));
+    const int rows = n * a.group;
+    return n == 0 ? 0.f : (float)(B::of_key(rows) * (keys + B::overhead(rows)));
   }
-  __device__ __forceinline__ void load(const PagedArgs& a, int from, long before, int lane) {
-    b0 = from;
-    mine = sequence(a, min(b0 + lane, a.batch - 1));
-    scan(a, before, lane);
+  __device__ __forceinline__ PagedLine line(const PagedArgs& a, int n, int keys) const {
+    if (way == kStretches) return weights(a, n, keys);
+    return paged_line_of_parts(way == kWhole ? 1 : paged_parts(heaviest(a, n, keys), per_length), n, a.group, B::rows_of_block(n * a.group));
   }
   __device__ __forceinline__ void scan(const PagedArgs& a, long before, int lane) {
     upto = before + scan_over_wave(b0 + lane < a.batch ? line(a, mine.n, mine.keys).all() * a.kv_head : 0);
   }
-  // Makes out the stretch of work group w; false if there is none.
-  //
-  // A stretch that ends where an item does costs one beginning less, so if there is a length for which all items have whole
-  // stretches, no more than kPagedGroups together, that is not longer by more than that, it is taken: of 64 lengths, from the even
-  // one up to three times that, by as many lanes.
+  __device__ __forceinline__ void load(const PagedArgs& a, int from, int lane) {
+    b0 = from;
+    mine = sequence(a, min(b0 + lane, a.batch - 1));
+  }
+  // Finds work group w's first item; false if it has none.
   __device__ __forceinline__ bool begin(const PagedArgs& a, int w, int lane) {
+    load(a, 0, lane);
+    long all = 0, count = 0;
+    float heavy = 0.f, light = -INFINITY;  // light: less than 0, the least weight
+    const bool one = a.batch <= 64;
+    for (int b = lane; b < a.batch; b += 64) {
+      const Sequence s = one ? mine : sequence(a, b);
+      const PagedLine t = weights(a, s.n, s.keys);
+      all += t.all() * a.kv_head;
+      count += (long)t.blocks * a.kv_head;
+      heavy = fmaxf(heavy, heaviest(a, s.n, s.keys));
+      if (s.n) light = fmaxf(light, -(float)t.of(0));
+    }
+    items = (int)of_lane(scan_over_wave(count), 63);
+    way = kWhole;
     per_length = 0.f;
-    load(a, 0, 0, lane);
-    long all = of_lane(upto, 63);
-    if (!a.shared) {
-      if (a.batch > 64) {
-        long more = 0;
-        for (int b = 64 + lane; b < a.batch; b += 64) {
-          const Sequence s = sequence(a, b);
-          more += line(a, s.n, s.keys).all() * a.kv_head;
+    length = 1, round = 0, stretch = 0;
+    if (a.shared) {
+      all = of_lane(scan_over_wave(all), 63);
+      heavy = same(max_over_wave(heavy));
+      const long even = paged_stretch(all);
+      const int rounds = (items + kPagedGroups - 1) >> kPagedGroupsLog;
+      light = -same(max_over_wave(light));
+      float best = rounds > 1 ? (float)rounds * ((float)all / (float)items)
+                              : fmaxf(B::kAlone * heavy, items <= kCus ? 0.f : 0.5f * (heavy + light));
+      if ((float)even + B::kStretchesCost < best) {
+        best = (float)even + B::kStretchesCost;
+        way = kStretches;
+        length = even;
+      }
+      if (one && items <= kPagedGroups) {
+        // 64 lengths, from the even one up to five times that, by as many lanes: the best for which there are stretches enough
+        const float mine_long = (float)even * (1.f + lane * (1.f / 16.f)), mine_in = 1.f / mine_long;
+        const float weight = heaviest(a, mine.n, mine.keys);
+        const int of_mine = weights(a, mine.n, mine.keys).blocks * a.kv_head;
+        int parts = 0;
+        for (int b = 0; b < a.batch; ++b)
+          parts += __builtin_amdgcn_readlane(of_mine, b) * paged_parts(__uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(weight), b)), mine_in);
+        const float cost = parts <= kCus ? B::kAlone * mine_long + 0.5f * B::kPartsCost : parts <= kPagedGroups ? mine_long + B::kPartsCost : INFINITY;
+        const float least = -same(max_over_wave(-cost));
+        if (least < best) {
+          const int l = __builtin_ctzll(__builtin_amdgcn_ballot_w64(cost == least));
+          way = kParts;
+          per_length = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(mine_in), l));
+          all = __builtin_amdgcn_readlane(parts, l);
+          length = 1;
         }
-        all += of_lane(scan_over_wave(more), 63);
-      }
-      length = 1;
-      stretch = paged_spread(w, (int)all);
-    } else if (a.batch > 64) {
-      long more = 0;
-      for (int b = 64 + lane; b < a.batch; b += 64) {
-        const Sequence s = sequence(a, b);
-        more += weights(a, s.n, s.keys).all() * a.kv_head;
-      }
-      all += of_lane(scan_over_wave(more), 63);
-      length = paged_stretch(all);
-      stretch = paged_spread(w, paged_stretches(all, length));
-    } else {
-      length = paged_stretch(all);
-      const float mine_in = 1.f / ((float)length * (1.f + lane * (1.f / 32.f)));
-      const float weight = heaviest(a, mine.n, mine.keys);
-      const int items = paged_blocks(mine.n * a.group, B::rows_of_block(mine.n * a.group)) * a.kv_head;
-      int parts = 0;
-      for (int b = 0; b < a.batch; ++b)
-        parts += __builtin_amdgcn_readlane(items, b) * paged_parts(__uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(weight), b)), mine_in);
-      const unsigned long long fit = __builtin_amdgcn_ballot_w64(parts <= kPagedGroups && (float)length * (lane * (1.f / 32.f)) <= B::kSecond);
-      if (fit) {
-        const int l = __builtin_ctzll(fit);
-        per_length = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(mine_in), l));
-        all = __builtin_amdgcn_readlane(parts, l);
-        length = 1;
-        scan(a, 0, lane);
-        stretch = paged_spread(w, (int)all);
-      } else {
-        stretch = paged_spread(w, paged_stretches(all, length));
       }
     }
-    x = stretch * length;
-    end = min(x + length, all);
-    return x < all;
+    way = (Way)same((int)way);
+    length = same(length);
+    scan(a, 0, lane);
+    if (way == kWhole) {
+      x = a.shared ? paged_whole(0, w, items) : w;
+      end = items;
+    } else {
+      stretch = same(paged_spread(w, way == kParts ? (int)all : paged_stretches(all, length)));
+      x = stretch * length;
+      end = same(min(x + length, all));
+    }
+    x = same(x);
+    return x < end;
   }
   __device__ __forceinline__ bool next(const PagedArgs& a, int lane, Part& r) {
     if (x >= end) return false;
     unsigned long long past;
     while (!(past = __builtin_amdgcn_ballot_w64(upto > x))) {
       if (b0 + 64 >= a.batch) return false;
-      load(a, b0 + 64, of_lane(upto, 63), lane);
+      const long before = of_lane(upto, 63);
+      load(a, b0 + 64, lane);
+      scan(a, before, lane);
     }
     const int l = __builtin_ctzll(past);
     r.b = b0 + l;
@@ -252,20 +284,36 @@ struct Walk {
     r.s.past = __builtin_amdgcn_readlane(mine.past, l);
     const PagedLine heads = line(a, r.s.n, r.s.keys);
     const long of_head = heads.all(), base = of_lane(upto, l) - of_head * a.kv_head;
-    r.head = __builtin_amdgcn_readfirstlane(paged_divide(x - base, of_head));
-    const long from = base + r.head * of_head;
-    r.block = heads.blocks == 1 ? 0 : __builtin_amdgcn_readfirstlane(paged_block_at(heads, x - from));
-    const long item = from + heads.before(r.block), weight = heads.of(r.block);
+    long item = 0, weight = 1;
+    if (way == kWhole) {
+      paged_whole_item((int)(x - base), heads.blocks, a.kv_head, r.block, r.head);
+      r.block = same(r.block), r.head = same(r.head);
+    } else {
+      r.head = same(paged_divide(x - base, of_head));
+      const long from = base + r.head * of_head;
+      r.block = heads.blocks == 1 ? 0 : same(paged_block_at(heads, x - from));
+      item = from + heads.before(r.block), weight = heads.of(r.block);
+    }
     const int rows = r.s.n * a.group, last = min(rows, (r.block + 1) * B::rows_of_block(rows)) - 1;
     const int tiles = paged_tiles(paged_visible(r.s.keys, r.s.n, last / a.group, a.causal));
-    r.t0 = __builtin_amdgcn_readfirstlane(paged_tile_at(tiles, x - item, weight));
-    r.t1 = __builtin_amdgcn_readfirstlane(paged_tile_at(tiles, end - item, weight));
-    r.opens = item >= x;
-    r.whole = r.opens && item + weight <= end;
-    r.parts = r.whole || !r.opens ? 1 : __builtin_amdgcn_readfirstlane(paged_divide(item + weight - 1, length)) - stretch + 1;
-    r.place = paged_place(stretch, r.opens ? 0 : 1) - (r.opens ? 0 : 2);
     r.stretch = stretch;
-    x = item + weight;
+    if (way == kWhole) {
+      r.t0 = 0, r.t1 = tiles;
+      r.opens = r.whole = true;
+      r.parts = 1, r.place = 0;
+      x = a.shared ? paged_whole(++round, blockIdx.x, items) : end;
+    } else {
+      r.t0 = paged_tile_at(tiles, x - item, weight);
+      r.t1 = paged_tile_at(tiles, end - item, weight);
+      r.opens = item >= x;
+      r.whole = r.opens && item + weight <= end;
+      r.parts = r.whole || !r.opens ? 1 : paged_divide(item + weight - 1, length) - stretch + 1;
+      r.place = paged_place(stretch, r.opens ? 0 : 1) - (r.opens ? 0 : 2);
+      x = item + weight;
+    }
+    x = same(x);
+    r.t0 = same(r.t0), r.t1 = same(r.t1), r.parts = same(r.parts), r.place = same(r.place);
+    r.opens = same((int)r.opens), r.whole = same((int)r.whole);
     return true;
   }
 };
@@ -815,8 +863,11 @@ __device__ __forceinline__ void many_rows(const PagedArgs& a, const Part& w, cha
     }
   };
 
-  // the block's rows of q fill the slots of V, which comes later
+  if (nt > 0) fetch_at(0);
+  // All that comes from memory first is asked for together: rows of q, pages, then K.  The rows of q go through the slots of V, which
+  // comes later.
   char* const my_rows = smem + kVOff + wave * (T::kBytes / 2);
+  u4v q_rows[2][T::kNC];
   {
     const int lane = lane_now(), r16 = lane >> 2, col = ((lane & 3) ^ swz(r16 >> 2)) * 16;
     const char* const base = a.q + w.b * a.q_batch + (a.ends ? w.s.first : 0) * a.q_seq + (long)w.head * (int)a.group * a.q_head;
@@ -825,12 +876,10 @@ __device__ __forceinline__ void many_rows(const PagedArgs& a, const Part& w, cha
       const int row = min(row0w + 16 * R + r16, rows - 1), token = row / a.group;
       const char* const from = base + token * a.q_seq + (row - token * (int)a.group) * a.q_head + col;
 #pragma unroll
-      for (int C = 0; C < T::kNC; ++C)
-        *reinterpret_cast<u4v*>(my_rows + T::block_off(R, C) + lane * 16) = *reinterpret_cast<const u4v*>(from + C * 64);
+      for (int C = 0; C < T::kNC; ++C) q_rows[R][C] = *reinterpret_cast<const u4v*>(from + C * 64);
     }
   }
   if (nt > 0) {
-    fetch_at(0);
     if constexpr (Q8) {
       unsigned k_sc1 = 0;
       ask_k(0, raw_k, k_sc);
@@ -847,6 +896,10 @@ __device__ __forceinline__ void many_rows(const PagedArgs& a, const Part& w, cha
       if (nt > 1) copy_k(1, lds_w + T::kBytes);
     }
   }
+#pragma unroll
+  for (int R = 0; R < 2; ++R)
+#pragma unroll
+    for (int C = 0; C < T::kNC; ++C) *reinterpret_cast<u4v*>(my_rows + T::block_off(R, C) + lane_now() * 16) = q_rows[R][C];
   h8 qf[G::kKSteps];
   {
     const StagedRows<D> staged{my_rows, lane_now()};
@@ -1254,9 +1307,13 @@ __global__ void __launch_bounds__(256) paged_join_kernel(PagedArgs a, int slot_r
   };
   const int row0 = blockIdx.x * rows_of_group;
   if (rows_of_group > 1) {
-    const int2 mine = place(row0 + slice);
-    if (!__syncthreads_or(mine.y > 2 * kJoinAhead)) {
-      if (mine.y > 1) store(row0 + slice, join_parts<D>(a, mine.x, mine.y, 0, 1, slot_rows, piece));
+    const int most = (int)threadIdx.x < rows_of_group ? place(row0 + threadIdx.x).y : 1;
+    if (!__syncthreads_or(most > 1)) return;
+    if (!__syncthreads_or(most > 2 * kJoinAhead)) {
+      for (int u = slice; u < rows_of_group; u += kSlices) {
+        const int2 at = place(row0 + u);
+        if (at.y > 1) store(row0 + u, join_parts<D>(a, at.x, at.y, 0, 1, slot_rows, piece));
+      }
       return;
     }
   }
@@ -1496,7 +1553,7 @@ template <int D, int FEW, bool MANY, bool BF, bool Q8>
 int launch_forward(const Launch& p, const PagedArgs& a, hipStream_t stream) {
   if (launch(paged_forward_kernel<D, FEW, MANY, BF, Q8>, dim3(p.grid()), kPagedThreads, stream, a) != hipSuccess) return FUSED_MHA_ERR_LAUNCH;
   if (!p.shared) return FUSED_MHA_OK;
-  const int rows = a.tokens * a.head, rows_of_group = MANY ? 256 / (D / 4) : 1;
+  const int rows = a.tokens * a.head, rows_of_group = MANY ? 32 : 1;
   return launch(paged_join_kernel<D, BF>, dim3((rows + rows_of_group - 1) / rows_of_group), 256, stream, a, p.place_rows(), rows_of_group) == hipSuccess
              ? FUSED_MHA_OK : FUSED_MHA_ERR_LAUNCH;
 }
@@ -1608,12 +1665,12 @@ int paged_mha_forward(const paged_mha_cache* c, const paged_mha_batch* b, const 
   a.q_batch = a.ends ? 0 : q_st->batch * 2, a.q_seq = q_st->seq * 2, a.q_head = q_st->head * 2;
   a.table_stride = b->table_stride;
   a.batch = b->batch, a.new_tokens = b->tokens, a.tokens = (int)all_tokens(b);
-  a.head = head, a.kv_head = c->kv_head, a.pages = c->pages, a.width = b->table_width;
+  a.head = head, a.kv_head = FmhaDivisor(c->kv_head), a.pages = c->pages, a.width = b->table_width;
   a.group = FmhaDivisor(head / c->kv_head), a.page_size = FmhaDivisor(c->page_size);
   a.c = scale * kLog2e;
   a.causal = causal != 0, a.zero_rest = zero_rest != 0 && a.ends;
   a.shared = p.shared;
-  a.step[0] = paged_step(p.few, head / c->kv_head), a.step[1] = paged_step(kManyRows, head / c->kv_head);
+  a.step[0] = paged_step(p.few, head / c->kv_head, p.many ? 2 : 4), a.step[1] = paged_step(kManyRows, head / c->kv_head, 4);
   if (p.many) fits(c, c->key_strides, bytes, a.k_shift), fits(c, c->value_strides, bytes, a.v_shift);
   return with_types(c, [&](auto d, auto bf, auto q8) {
     constexpr int D = decltype(d)::value;

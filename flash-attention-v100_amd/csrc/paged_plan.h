@@ -5,11 +5,15 @@
 #include "block_map.h"
 
 // Rows of a sequence and key head: its new tokens times the query heads of the key head, token by token.  A block is a number
-// of neighbouring rows, an item a block of one sequence and key head with the tiles of keys that it sees.  Items stand in a
-// line, sequence by sequence, key head by key head, block by block, each as long as its work (its weight), and each work group
-// gets a stretch of the line of the same length: the end of an item that begins in an earlier stretch, whole items, and the
-// beginning of one that goes on in the next.  An item that lies in several stretches is joined afterwards, part by part.
-// All work groups have the same amount of work whatever the lengths are, and none needs to know what others do.
+// of neighbouring rows, an item a block of one sequence and key head with the tiles of keys that it sees.  kPagedGroups work groups
+// share the items in one of three ways, whichever takes the longest of them the least time; none needs to know what others do:
+//
+//   stretches  Items stand in a line, sequence by sequence, key head by key head, block by block, each as long as its work (its
+//              weight), and each work group gets a stretch of the line of the same length: the end of an item that begins in an
+//              earlier stretch, whole items, and the beginning of one that goes on in the next.  An item that lies in several
+//              stretches is joined afterwards, part by part.
+//   parts      The same with items rounded up to whole stretches, so that none begins inside of one.
+//   whole      Items in rounds, the ones that see most first, key heads next to each other; nothing to join.
 constexpr int kPagedTile = 64;  // keys
 
 FMHA_HOST_DEVICE int paged_tiles(int keys) { return (keys + kPagedTile - 1) / kPagedTile; }
@@ -30,13 +34,13 @@ struct PagedLine {
   FMHA_HOST_DEVICE long of(int k) const { return first + (long)step * (k + 1); }
   FMHA_HOST_DEVICE long all() const { return before(blocks); }
 };
-// In quarters of a key: about the keys that a block sees, and something for its beginning and end.  step: 0 without a causal mask,
-// else paged_step, which divides.
-FMHA_HOST_DEVICE int paged_step(int rows_of_block, int group) { return 4 * rows_of_block / group; }
+// About the keys that a block sees, and something for its beginning and end, times the weight of a key.  step: 0 without a causal
+// mask, else paged_step, which divides.
+FMHA_HOST_DEVICE int paged_step(int rows_of_block, int group, int of_key) { return of_key * rows_of_block / group; }
 template <typename Int>  // int or FmhaDivisor
-FMHA_HOST_DEVICE PagedLine paged_line(int keys, int new_tokens, const Int& group, int step, int rows_of_block, int overhead) {
+FMHA_HOST_DEVICE PagedLine paged_line(int keys, int new_tokens, const Int& group, int step, int rows_of_block, int overhead, int of_key) {
   const int hidden = step == 0 ? 0 : new_tokens < keys ? new_tokens : keys;
-  return PagedLine{4 * (long)(keys - hidden + overhead), step, paged_blocks(new_tokens * group, rows_of_block)};
+  return PagedLine{of_key * (long)(keys - hidden + overhead), step, paged_blocks(new_tokens * group, rows_of_block)};
 }
 // In stretches, where every item has a whole number of them.
 template <typename Int>
@@ -84,6 +88,19 @@ FMHA_HOST_DEVICE int paged_tile_at(int tiles, long into, long weight) {
   if (into >= weight) return tiles;
   const int at = (int)((float)into * ((float)tiles / (float)weight));  // grows with `into`, the same on both sides
   return at < tiles ? at : tiles;
+}
+
+// Item that work group w takes in a round of whole ones: as the persistent kernels for equal lengths, or, if there is one round only,
+// as those of which two share a CU.
+FMHA_HOST_DEVICE int paged_whole(int round, int w, int items) {
+  return items <= kPagedGroups ? round == 0 && w < items ? fmha_paired_block(w, items) : items : fmha_persistent_block(round, w, kPagedGroups);
+}
+// Item `at` of a sequence's: its block, the last one first, and key head.
+template <typename Int>
+FMHA_HOST_DEVICE void paged_whole_item(int at, int blocks, const Int& kv_heads, int& block, int& head) {
+  const int level = at / kv_heads;
+  block = blocks - 1 - level;
+  head = at - level * (int)kv_heads;
 }
 
 // Work group w of a launch has stretch paged_spread(w, stretches), if that is one: neighbouring stretches, which read the same keys,

@@ -276,7 +276,7 @@ int main() {
     long all = 0;
     for (int b = 0; b < batch; ++b) {
       seqs[b] = {rnd(3) ? rnd(3) : rnd(300), rnd(3) ? rnd(500) : rnd(20000)};
-      lines[b] = ones ? paged_line_of_parts(1 + rnd(5), seqs[b].n, group, rows_of_block) : paged_line(seqs[b].keys, seqs[b].n, group, causal ? paged_step(rows_of_block, group) : 0, rows_of_block, 64);
+      lines[b] = ones ? paged_line_of_parts(1 + rnd(5), seqs[b].n, group, rows_of_block) : paged_line(seqs[b].keys, seqs[b].n, group, causal ? paged_step(rows_of_block, group, 4) : 0, rows_of_block, 64, 4);
       all += lines[b].all() * kv;
     }
     const long length = ones ? 1 : paged_stretch(all);
@@ -357,6 +357,39 @@ int main() {
     for (int p = 0; p < parts; ++p)
       if (taken[p] != 1) return puts("not once"), 1;
   }
+  puts("ok");
+}
+""")
+    assert out == "ok\n"
+
+
+def test_whole_items_are_taken_once(tmp_path):
+    out = host_program(tmp_path, r"""
+int main() {
+  for (int items = 0; items < 6000; items += items < 700 ? 1 : 37) {
+    std::vector<int> taken(items);
+    for (int w = 0; w < kPagedGroups; ++w) {
+      int last = -1;
+      for (int round = 0;; ++round) {
+        const int at = paged_whole(round, w, items);
+        if (at >= items) break;
+        if (at <= last) return puts("back"), 1;
+        last = at;
+        ++taken[at];
+      }
+    }
+    for (int t : taken)
+      if (t != 1) return puts("not once"), 1;
+  }
+  for (int blocks = 1; blocks < 20; ++blocks)
+    for (int heads = 1; heads < 20; ++heads) {
+      std::vector<int> taken(blocks * heads);
+      for (int at = 0; at < blocks * heads; ++at) {
+        int block, head;
+        paged_whole_item(at, blocks, FmhaDivisor(heads), block, head);
+        if (block < 0 || block >= blocks || head < 0 || head >= heads || taken[block * heads + head]++) return puts("item"), 1;
+      }
+    }
   puts("ok");
 }
 """)
