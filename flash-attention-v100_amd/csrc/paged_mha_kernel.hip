@@ -152,8 +152,8 @@ struct Blocks {
   static __device__ __forceinline__ int of_key(int rows) { return MANY && FEW && !many(rows) ? 2 : 4; }
   // A block of many rows alone on its CU takes 0.55 of the time.  What parts cost (256: a tile): an item more in a stretch, and of
   // many rows to write their sums and to read them again, of up to two in each stretch or of one.
-  static constexpr float kAlone = MANY ? 0.55f : 1.f;
-  static constexpr float kStretchesCost = (MANY ? 3 + 14 : 1) * 256, kPartsCost = MANY ? 7 * 256 : 0;
+  static constexpr float kAlone = MANY ? 0.58f : 1.f;
+  static constexpr float kStretchesCost = (MANY ? 3 + 14 : 1) * 256, kPartsCost = MANY ? 6 * 256 : 0;
 };
 // What a work group does of an item.
 struct Part {
@@ -848,23 +848,39 @@ __device__ __forceinline__ void many_rows(const PagedArgs& a, const Part& w, cha
   };
   // Of a lane's 16 values one half is chunk c, the other c ^ 1 of a row; lanes two apart write the same banks, so they begin with
   // different halves.
-  auto put = [&](unsigned raw, unsigned sc, unsigned tile) __attribute__((always_inline)) {
-    typedef __attribute__((address_space(3))) u2v lds_u2v;
-    typedef __attribute__((address_space(3))) u4v lds_u4v;
-    const int lane = lane_now(), r16 = lane >> 2, q4 = lane & 3, half = q4 >> 1;
-    const unsigned from = raw + lane * 16 + half * 8;
-    const unsigned to = tile + T::block_off(wave, half) + r16 * 64 + (((2 * (q4 & 1) + half) ^ swz(r16 >> 2)) * 16);
-    const float scale = scale_of(sc);
+  typedef __attribute__((address_space(3))) u2v lds_u2v;
+  typedef __attribute__((address_space(3))) u4v lds_u4v;
+  struct Put {
+    unsigned from[2], to[2];  // the lane's halves of raw rows of K and its chunks of the first tile, the half that it begins with first
+  };
+  auto put_lane = [&]() __attribute__((always_inline)) {
+    const int lane = lane_now(), r16 = lane >> 2, q4 = lane & 3, first = q4 >> 1;
+    Put p;
+    p.from[0] = raw_k + lane * 16 + first * 8;
+    p.to[0] = lds0 + T::block_off(wave, first) + r16 * 64 + (((2 * (q4 & 1) + first) ^ swz(r16 >> 2)) * 16);
+    p.from[1] = p.from[0] ^ 8, p.to[1] = p.to[0] ^ 16;
+#pragma unroll
+    for (int half = 0; half < 2; ++half) asm volatile("" : "+v"(p.from[half]), "+v"(p.to[half]));
+    return p;
+  };
+  auto put_from = [&](const Put& p, bool value, int i, int half) __attribute__((always_inline)) {
+    return *(const lds_u2v*)(uintptr_t)(p.from[half] + (value ? M::kRaw : 0) + 1024 * i);
+  };
+  auto put_to = [&](const Put& p, unsigned tile, u2v x, float scale, int i, int half) __attribute__((always_inline)) {
+    *(lds_u4v*)(uintptr_t)(p.to[half] + tile + T::block_off(0, 2 * i)) = from_e4m3<BF>(x[0], x[1], scale);
+  };
+  auto put = [&](bool value, unsigned sc, unsigned tile) __attribute__((always_inline)) {
+    const Put p = put_lane();
 #pragma unroll
     for (int i = 0; i < kCopies; ++i) {
-      const u2v x = *(const lds_u2v*)(uintptr_t)(from + 1024 * i), y = *(const lds_u2v*)(uintptr_t)((from ^ 8) + 1024 * i);
-      *(lds_u4v*)(uintptr_t)(to + T::block_off(0, 2 * i)) = from_e4m3<BF>(x[0], x[1], scale);
-      *(lds_u4v*)(uintptr_t)((to ^ 16) + T::block_off(0, 2 * i)) = from_e4m3<BF>(y[0], y[1], scale);
+      const u2v x = put_from(p, value, i, 0), y = put_from(p, value, i, 1);
+      put_to(p, tile, x, scale_of(sc), i, 0);
+      put_to(p, tile, y, scale_of(sc), i, 1);
     }
   };
 
   if (nt > 0) fetch_at(0);
-  // All that comes from memory first is asked for together: rows of q, pages, then K.  The rows of q go through the slots of V, which
+  // All that comes from memory first is asked for together: pages, rows of q, then K.  The rows of q go through the slots of V, which
   // comes later.
   char* const my_rows = smem + kVOff + wave * (T::kBytes / 2);
   u4v q_rows[2][T::kNC];
@@ -886,8 +902,8 @@ __device__ __forceinline__ void many_rows(const PagedArgs& a, const Part& w, cha
       if (nt > 1) ask_k(1, raw_v, k_sc1);
       wait_vm<0>();
       asm volatile("" ::: "memory");
-      put(raw_k, k_sc, lds0);
-      if (nt > 1) put(raw_v, k_sc1, lds0 + T::kBytes);
+      put(false, k_sc, 0);
+      if (nt > 1) put(true, k_sc1, T::kBytes);
       staged_rows_read();
       if (nt > 2) ask_k(2, raw_k, k_sc);
       ask_v(0);
@@ -1018,13 +1034,13 @@ __device__ __forceinline__ void many_rows(const PagedArgs& a, const Part& w, cha
   };
   auto next_k = [&](int j, int slot) __attribute__((always_inline)) {
     if constexpr (Q8) {
-      if (j + 2 < nt) put(raw_k, k_sc, lds0 + slot * T::kBytes);
+      if (j + 2 < nt) put(false, k_sc, slot * T::kBytes);
     } else {
       if (j + 2 < nt) copy_k(j + 2, lds_w + slot * T::kBytes);
     }
   };
   auto next_v = [&](int j, int slot) __attribute__((always_inline)) {
-    if constexpr (Q8) put(raw_v, v_sc, lds0 + kVOff + slot * T::kBytes);
+    if constexpr (Q8) put(true, v_sc, kVOff + slot * T::kBytes);
     else copy_v(j, lds_w + kVOff + slot * T::kBytes);
   };
   auto ask = [&](int j) __attribute__((always_inline)) {
@@ -1045,6 +1061,9 @@ __device__ __forceinline__ void many_rows(const PagedArgs& a, const Part& w, cha
     constexpr unsigned at = kSlot * T::kBytes;
     constexpr int kM = kNS + kNP;
     h8 frag[kLead];
+    u2v raw[Q8 ? 2 * kCopies : 1];
+    Put where;
+    if constexpr (Q8) where = put_lane();
     float l0 = 0.f, l1 = 0.f, p0 = 0.f, p1 = 0.f;
     auto read = [&](int m) __attribute__((always_inline)) {
       const int ch = m / (2 * kDB), in = m % (2 * kDB);
@@ -1065,20 +1084,35 @@ __device__ __forceinline__ void many_rows(const PagedArgs& a, const Part& w, cha
     };
     top_wait();
     fetch_for(j);
-    if constexpr (Q8) {
-      next_v(j, 1 - kSlot);
-      next_k(j, 1 - kSlot);
-      ask(j);
-    }
 #pragma unroll
     for (int m = 0; m < kLead; ++m) frag[m] = read(m);
     constexpr int kCopyKAt = Q8 ? -1 : D == 128 ? 8 : 0;  // K's copies follow when V's are through
     if (!Q8) next_v(j, 1 - kSlot);
     if (kCopyKAt == 0) next_k(j, 1 - kSlot);
     __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-    for (int m = 0; m < kM + 2; ++m) {
+    static_for<kM + 2>([&](auto m_tag) __attribute__((always_inline)) {
+      constexpr int m = decltype(m_tag)::value;
       if (kCopyKAt != 0 && m == kCopyKAt) next_k(j, 1 - kSlot);
+      if constexpr (Q8) {  // V's halves of 16 rows, then K's, one every other unit; the next are asked for as soon as they are read
+        constexpr int kHalves = 2 * kCopies;
+        constexpr int kVFirst = 4, kVEnd = kVFirst + 2 * kHalves, kKFirst = kVEnd + 2, kKEnd = kKFirst + 2 * kHalves;
+        if constexpr (m == 0 || m == kVEnd - 1) {
+#pragma unroll
+          for (int n = 0; n < kHalves; ++n) raw[n] = put_from(where, m == 0, n / 2, n % 2);
+        }
+        if constexpr (m >= kVFirst && m < kVEnd && m % 2 == 0) {
+          constexpr int h = (m - kVFirst) / 2;
+          put_to(where, kVOff + (1 - kSlot) * T::kBytes, raw[h], scale_of(v_sc), h / 2, h % 2);
+        }
+        if constexpr (m >= kKFirst && m < kKEnd && m % 2 == 0) {
+          constexpr int h = (m - kKFirst) / 2;
+          put_to(where, (1 - kSlot) * T::kBytes, raw[h], scale_of(k_sc), h / 2, h % 2);
+        }
+        if constexpr (m == kKEnd) {
+          if (j + 3 < nt) ask_k(j + 3, raw_k, k_sc);
+          if (j + 1 < nt) ask_v(j + 1);
+        }
+      }
       if (m < kM && m % 2 == 0) {  // one wait for the fragments of this unit and the next
         if (D == 64) wait_lds_pinned(reads(m + 2));
         else wait_lds(reads(m + 2));
@@ -1104,7 +1138,7 @@ __device__ __forceinline__ void many_rows(const PagedArgs& a, const Part& w, cha
         }
       }
       __builtin_amdgcn_sched_barrier(0);
-    }
+    });
     return l0 + l1;
   };
 
