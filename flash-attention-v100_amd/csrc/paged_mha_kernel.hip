@@ -1093,19 +1093,19 @@ __device__ __forceinline__ void many_rows(const PagedArgs& a, const Part& w, cha
     static_for<kM + 2>([&](auto m_tag) __attribute__((always_inline)) {
       constexpr int m = decltype(m_tag)::value;
       if (kCopyKAt != 0 && m == kCopyKAt) next_k(j, 1 - kSlot);
-      if constexpr (Q8) {  // V's halves of 16 rows, then K's, one every other unit; the next are asked for as soon as they are read
+      if constexpr (Q8) {  // V's halves of 16 rows, then K's, one with every unit; the next are asked for as soon as these are read
         constexpr int kHalves = 2 * kCopies;
-        constexpr int kVFirst = 4, kVEnd = kVFirst + 2 * kHalves, kKFirst = kVEnd + 2, kKEnd = kKFirst + 2 * kHalves;
-        if constexpr (m == 0 || m == kVEnd - 1) {
+        constexpr int kVFirst = 2, kVEnd = kVFirst + kHalves, kKFirst = kVEnd + 2, kKEnd = kKFirst + kHalves;
+        if constexpr (m == 0 || m == kVEnd) {
 #pragma unroll
           for (int n = 0; n < kHalves; ++n) raw[n] = put_from(where, m == 0, n / 2, n % 2);
         }
-        if constexpr (m >= kVFirst && m < kVEnd && m % 2 == 0) {
-          constexpr int h = (m - kVFirst) / 2;
+        if constexpr (m >= kVFirst && m < kVEnd) {
+          constexpr int h = m - kVFirst;
           put_to(where, kVOff + (1 - kSlot) * T::kBytes, raw[h], scale_of(v_sc), h / 2, h % 2);
         }
-        if constexpr (m >= kKFirst && m < kKEnd && m % 2 == 0) {
-          constexpr int h = (m - kKFirst) / 2;
+        if constexpr (m >= kKFirst && m < kKEnd) {
+          constexpr int h = m - kKFirst;
           put_to(where, (1 - kSlot) * T::kBytes, raw[h], scale_of(k_sc), h / 2, h % 2);
         }
         if constexpr (m == kKEnd) {
