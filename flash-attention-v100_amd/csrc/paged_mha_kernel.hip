@@ -416,28 +416,30 @@ __device__ __forceinline__ void few_rows(const PagedArgs& a, const Part& w, char
   const int units = min(2 * w.t1, (seen + kUnit - 1) / kUnit) - 2 * t0;  // of the part
   const int u0 = 2 * t0 + max(units, 0) * wave / kFewWaves, u1 = 2 * t0 + max(units, 0) * (wave + 1) / kFewWaves;
 
-  // page numbers of 64 stretches of 16 positions, from stretch ids0 on
+  // Where 64 stretches of 16 positions lie in the cache, lane l's being stretch from + l; behind the last one it is that one.
   bool bad = w.s.past;
-  int ids = 0, ids0 = 0;
-  auto fetch_ids = [&](int stretch0) __attribute__((always_inline)) {
-    ids0 = stretch0;
-    const int at = min((stretch0 + lane) * 16, w.s.keys - 1);
-    ids = a.table[w.b * a.table_stride + at / a.page_size];
-    const bool none = (unsigned)ids >= (unsigned)a.pages;
+  const int last_stretch = (w.s.keys - 1) >> 4;
+  int from = 0;
+  long k_at = 0, v_at = 0, ks_at = 0, vs_at = 0;
+  auto fetch = [&](int first) __attribute__((always_inline)) {
+    from = first;
+    const int pos = min(first + lane, last_stretch) * 16, page_at = pos / a.page_size, slot = pos - page_at * (int)a.page_size;
+    int id = a.table[w.b * a.table_stride + page_at];
+    const bool none = (unsigned)id >= (unsigned)a.pages;
     // of stretches that are behind the wave's last one nothing is said
-    bad |= __builtin_amdgcn_ballot_w64(none && stretch0 + lane < 2 * u1) != 0;
-    if (none) ids = 0;
+    bad |= __builtin_amdgcn_ballot_w64(none && first + lane < 2 * u1) != 0;
+    if (none) id = 0;
+    k_at = id * a.ks.page + (long)slot * a.ks.slot;
+    v_at = id * a.vs.page + (long)slot * a.vs.slot;
+    if constexpr (Q8) {
+      ks_at = id * a.kss.page + (long)slot * a.kss.slot;
+      vs_at = id * a.vss.page + (long)slot * a.vss.slot;
+    }
   };
-  if (u0 < u1) fetch_ids(2 * u0);
-  // Positions 16 R .. of unit u: their page, the first's slot, and how many there are less one.  Those past the last key are it again.
-  struct Stretch {
-    long id;
-    int slot, last;
-  };
-  auto stretch_of = [&](int u, int R) __attribute__((always_inline)) {
-    const int stretch = min(2 * u + R, (w.s.keys - 1) >> 4), pos = stretch * 16, page_at = pos / a.page_size;
-    return Stretch{__builtin_amdgcn_readlane(ids, stretch - ids0), pos - page_at * (int)a.page_size, w.s.keys - 1 - pos};
-  };
+  if (u0 < u1) fetch(2 * u0);
+  // stretch R of unit u: the lane that has it, and how many positions it has, less one
+  auto lane_of = [&](int u, int R) __attribute__((always_inline)) { return min(2 * u + R, last_stretch) - from; };
+  auto last_of = [&](int u, int R) __attribute__((always_inline)) { return w.s.keys - 1 - min(2 * u + R, last_stretch) * 16; };
 
   h8 qf[CB][kKS];
   int sees[CB];  // keys that the lane's row of a column block sees
@@ -468,6 +470,7 @@ __device__ __forceinline__ void few_rows(const PagedArgs& a, const Part& w, char
 #pragma unroll
     for (int e = 0; e < 8; ++e) t[e] = s[e >> 2][e & 3] * a.c;
     if (u * kUnit + kUnit > all_see) {
+      asm volatile("");  // stays a branch
       const int left = sees[cb] - u * kUnit - 16 * (g >> 1) - 4 * (g & 1);
 #pragma unroll
       for (int e = 0; e < 8; ++e)
@@ -490,18 +493,23 @@ __device__ __forceinline__ void few_rows(const PagedArgs& a, const Part& w, char
     const int col = (q4 ^ swz(r16 >> 2)) * 16;
     char* const v_tile = tile + G::kTileBytes;
     u4v kr[2][kLoads], vr[2][kLoads];
+    const int k_lane = r16 * a.ks.slot + col, v_lane = r16 * a.vs.slot + col;
     auto load = [&](int u) __attribute__((always_inline)) {
-      if (2 * u - ids0 >= 64) fetch_ids(2 * u);
+      if (2 * u - from >= 64) fetch(2 * u);
 #pragma unroll
       for (int R = 0; R < 2; ++R) {
-        const Stretch t = stretch_of(u, R);
-        const int r = min(r16, t.last);
-        const char* const kb = k_head + t.id * a.ks.page + (long)t.slot * a.ks.slot;
-        const char* const vb = v_head + t.id * a.vs.page + (long)t.slot * a.vs.slot;
+        const char* const kb = k_head + of_lane(k_at, lane_of(u, R));
+        const char* const vb = v_head + of_lane(v_at, lane_of(u, R));
+        int ko = k_lane, vo = v_lane;
+        if (last_of(u, R) < 15) {  // positions past the last one: the last one again
+          asm volatile("");
+          const int past = max(r16 - last_of(u, R), 0);
+          ko -= past * a.ks.slot, vo -= past * a.vs.slot;
+        }
 #pragma unroll
-        for (int i = 0; i < kLoads; ++i) kr[R][i] = *reinterpret_cast<const u4v*>(kb + (unsigned)(r * a.ks.slot + col + 64 * i));
+        for (int i = 0; i < kLoads; ++i) kr[R][i] = *reinterpret_cast<const u4v*>(kb + (unsigned)(ko + 64 * i));
 #pragma unroll
-        for (int i = 0; i < kLoads; ++i) vr[R][i] = *reinterpret_cast<const u4v*>(vb + (unsigned)(r * a.vs.slot + col + 64 * i));
+        for (int i = 0; i < kLoads; ++i) vr[R][i] = *reinterpret_cast<const u4v*>(vb + (unsigned)(vo + 64 * i));
       }
     };
     const unsigned ka0 = opaque_lds_address(tile + rows16_off<D>(lane, 0)), ka1 = opaque_lds_address(tile + rows16_off<D>(lane, 1));
@@ -518,14 +526,22 @@ __device__ __forceinline__ void few_rows(const PagedArgs& a, const Part& w, char
       }
       if (u + 1 < u1) load(u + 1);
       f4v s[CB][2];
+      h8 frag[2 * kKS];  // asked for together, and again those of V in front of the exponentials
 #pragma unroll
-      for (int kk = 0; kk < kKS; ++kk) {
+      for (int n = 0; n < 2 * kKS; ++n) frag[n] = rows16_at<D>(ka0, ka1, n & 1, n >> 1);
+      __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-        for (int p = 0; p < 2; ++p) {
-          const h8 kf = rows16_at<D>(ka0, ka1, p, kk);
+      for (int n = 0; n < 2 * kKS; ++n) {
+        const int p = n & 1, kk = n >> 1;
 #pragma unroll
-          for (int cb = 0; cb < CB; ++cb) s[cb][p] = mma16<BF>(kf, qf[cb][kk], kk == 0 ? f4v{0.f, 0.f, 0.f, 0.f} : s[cb][p]);
-        }
+        for (int cb = 0; cb < CB; ++cb) s[cb][p] = mma16<BF>(frag[n], qf[cb][kk], kk == 0 ? f4v{0.f, 0.f, 0.f, 0.f} : s[cb][p]);
+      }
+      static_assert(kDB == 2 * kKS, "");
+      if (CB == 1) {
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int db = 0; db < kDB; ++db) frag[db] = va.at(0, 0, db);
+        __builtin_amdgcn_sched_barrier(0);
       }
       u4v pf[CB];
       float alpha[CB];
@@ -553,7 +569,7 @@ __device__ __forceinline__ void few_rows(const PagedArgs& a, const Part& w, char
       }
 #pragma unroll
       for (int db = 0; db < kDB; ++db) {
-        const h8 vf = va.at(0, 0, db);
+        const h8 vf = CB == 1 ? frag[db] : va.at(0, 0, db);
 #pragma unroll
         for (int cb = 0; cb < CB; ++cb) o[cb][db] = mma16<BF>(vf, __builtin_bit_cast(h8, pf[cb]), o[cb][db]);
       }
@@ -573,35 +589,42 @@ __device__ __forceinline__ void few_rows(const PagedArgs& a, const Part& w, char
       if constexpr (kLoads == 1) copy16(wave_uniform(from), off, smem + __builtin_amdgcn_readfirstlane(to - lds0) + wave * G::kWaveBytes);
       else copy16_blocks<kLoads>(wave_uniform(from - kBack), off + kBack, __builtin_amdgcn_readfirstlane(to));
     };
+    const int k_lane = r16 * a.ks.slot, v_lane = r16 * a.vs.slot;
+    // scales of the 32 keys, then of the values, a lane each
+    const unsigned char* const sc_head = lane < 32 ? a.k_scale + (long)w.head * a.kss.head : a.v_scale + (long)w.head * a.vss.head;
+    const int sc_slot = lane < 32 ? a.kss.slot : a.vss.slot;
     auto ask = [&](int u, unsigned slot) __attribute__((always_inline)) {
-      if (2 * u - ids0 >= 64) fetch_ids(2 * u);
-      const Stretch t[2] = {stretch_of(u, 0), stretch_of(u, 1)};
+      if (2 * u - from >= 64) fetch(2 * u);
+      int sc_row = lane & 15;
 #pragma unroll
       for (int R = 0; R < 2; ++R) {
-        const int r = min(r16, t[R].last), at = R * kLoads * 1024;
-        copy(k_head + t[R].id * a.ks.page + (long)t[R].slot * a.ks.slot, r * a.ks.slot + (col ^ (32 * R)), slot + at);
-        copy(v_head + t[R].id * a.vs.page + (long)t[R].slot * a.vs.slot, r * a.vs.slot + (col ^ (32 * R)), slot + G::kTileBytes + at);
+        int ko = k_lane + (col ^ (32 * R)), vo = v_lane + (col ^ (32 * R));
+        if (last_of(u, R) < 15) {  // positions past the last one: the last one again
+          asm volatile("");
+          const int past = max(r16 - last_of(u, R), 0);
+          ko -= past * a.ks.slot, vo -= past * a.vs.slot;
+          if ((lane >> 4 & 1) == R) sc_row = min(sc_row, last_of(u, R));
+        }
+        copy(k_head + of_lane(k_at, lane_of(u, R)), ko, slot + R * kLoads * 1024);
+        copy(v_head + of_lane(v_at, lane_of(u, R)), vo, slot + G::kTileBytes + R * kLoads * 1024);
       }
-      // scales of the 32 keys, then of the values
-      const bool R = lane & 16;
-      const long id = R ? t[1].id : t[0].id, at = (R ? t[1].slot : t[0].slot) + min(lane & 15, R ? t[1].last : t[0].last);
-      const unsigned char* const ks = a.k_scale + (long)w.head * a.kss.head + id * a.kss.page + at * a.kss.slot;
-      const unsigned char* const vs = a.v_scale + (long)w.head * a.vss.head + id * a.vss.page + at * a.vss.slot;
-      copy_byte(lane < 32 ? ks : vs, __builtin_amdgcn_readfirstlane(slot + 2 * G::kTileBytes));
+      const long ks = lane & 16 ? of_lane(ks_at, lane_of(u, 1)) : of_lane(ks_at, lane_of(u, 0));
+      const long vs = lane & 16 ? of_lane(vs_at, lane_of(u, 1)) : of_lane(vs_at, lane_of(u, 0));
+      copy_byte(sc_head + (lane < 32 ? ks : vs) + (long)sc_row * sc_slot, __builtin_amdgcn_readfirstlane(slot + 2 * G::kTileBytes));
     };
-    unsigned k_at[2];  // the lane's row of keys: 8 p + (m & 7) of rows 16 (m >> 3) ..
-    unsigned k_at_scale[2], v_at_scale[2];
+    unsigned k_row[2];  // the lane's row of keys: 8 p + (m & 7) of rows 16 (m >> 3) ..
+    unsigned k_scale_at[2], v_scale_at[2];
 #pragma unroll
     for (int p = 0; p < 2; ++p) {
       const int R = m >> 3, row = 8 * p + (m & 7);
-      k_at[p] = lds0 + R * kLoads * 1024 + row * 64 + (((g >> 1) ^ swz(row >> 2) ^ (2 * R)) * 16) + (g & 1) * 8;
-      k_at_scale[p] = lds0 + 2 * G::kTileBytes + (16 * R + row) * 4;
-      v_at_scale[p] = lds0 + 2 * G::kTileBytes + (32 + 16 * (g >> 1) + 8 * p + 4 * (g & 1)) * 4;
+      k_row[p] = lds0 + R * kLoads * 1024 + row * 64 + (((g >> 1) ^ swz(row >> 2) ^ (2 * R)) * 16) + (g & 1) * 8;
+      k_scale_at[p] = lds0 + 2 * G::kTileBytes + (16 * R + row) * 4;
+      v_scale_at[p] = lds0 + 2 * G::kTileBytes + (32 + 16 * (g >> 1) + 8 * p + 4 * (g & 1)) * 4;
     }
-    unsigned v_at;  // of 8 keys of the lane's group, in the order of its probabilities, a pair of lanes has 16 features of each
+    unsigned v_row;  // of 8 keys of the lane's group, in the order of its probabilities, a pair of lanes has 16 features of each
     {
       const int R = g >> 1, row = 4 * (g & 1) + (m >> 1 & 3) + 8 * (m >> 3);
-      v_at = lds0 + G::kTileBytes + R * kLoads * 1024 + row * 64 + ((swz(row >> 2) ^ (2 * R)) * 16) + (m & 1) * 8;
+      v_row = lds0 + G::kTileBytes + R * kLoads * 1024 + row * 64 + ((swz(row >> 2) ^ (2 * R)) * 16) + (m & 1) * 8;
     }
     if (u0 < u1) ask(u0, lds0);
     if (u0 + 1 < u1) ask(u0 + 1, lds0 + G::kSlotBytes);
@@ -611,24 +634,34 @@ __device__ __forceinline__ void few_rows(const PagedArgs& a, const Part& w, char
       else wait_vm<0>();
       asm volatile("" ::: "memory");
       f4v s[CB][2];
+      // asked for together: scales, K, and in front of the exponentials V
+      float scale[2];
+      u4v e4[2];
+      u2v frag[2 * kKS];
 #pragma unroll
-      for (int p = 0; p < 2; ++p) {
-        const float scale = scale_of(*(const lds_u*)(uintptr_t)(k_at_scale[p] + slot));
+      for (int p = 0; p < 2; ++p) scale[p] = scale_of(*(const lds_u*)(uintptr_t)(k_scale_at[p] + slot));
 #pragma unroll
-        for (int kk = 0; kk < kKS; ++kk) {
-          const u2v x = *(const lds_u2v*)(uintptr_t)(((k_at[p] + slot) ^ (kk & 1) * 32) + (kk >> 1) * 1024);
-          const h8 kf = __builtin_bit_cast(h8, from_e4m3<BF>(x[0], x[1], scale));
+      for (int n = 0; n < 2 * kKS; ++n)
+        frag[n] = *(const lds_u2v*)(uintptr_t)(((k_row[n & 1] + slot) ^ (n >> 1 & 1) * 32) + (n >> 2) * 1024);
 #pragma unroll
-          for (int cb = 0; cb < CB; ++cb) s[cb][p] = mma16<BF>(kf, qf[cb][kk], kk == 0 ? f4v{0.f, 0.f, 0.f, 0.f} : s[cb][p]);
-        }
+      for (int p = 0; p < 2; ++p) e4[p] = *(const lds_u4v*)(uintptr_t)(v_scale_at[p] + slot);
+      __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+      for (int n = 0; n < 2 * kKS; ++n) {
+        const int p = n & 1, kk = n >> 1;
+        const h8 kf = __builtin_bit_cast(h8, from_e4m3<BF>(frag[n][0], frag[n][1], scale[p]));
+#pragma unroll
+        for (int cb = 0; cb < CB; ++cb) s[cb][p] = mma16<BF>(kf, qf[cb][kk], kk == 0 ? f4v{0.f, 0.f, 0.f, 0.f} : s[cb][p]);
       }
+      static_assert(kDB == 2 * kKS, "");
+      __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+      for (int db = 0; db < kDB; ++db)
+        frag[db] = __builtin_bit_cast(u2v, __builtin_amdgcn_ds_read_tr8_b64_v2i32((lds_i2v*)(uintptr_t)(((v_row + slot) ^ (db & 3) * 16) + (db >> 2) * 1024)));
+      __builtin_amdgcn_sched_barrier(0);
       float e8[8];  // exponents of the lane's values
 #pragma unroll
-      for (int p = 0; p < 2; ++p) {
-        const u4v x = *(const lds_u4v*)(uintptr_t)(v_at_scale[p] + slot);
-#pragma unroll
-        for (int r = 0; r < 4; ++r) e8[4 * p + r] = (float)(int)(x[r] - 127);
-      }
+      for (int e = 0; e < 8; ++e) e8[e] = (float)(int)(e4[e >> 2][e & 3] - 127);
       u4v pf[CB];
       float alpha[CB];
       bool moved = false;
@@ -655,8 +688,7 @@ __device__ __forceinline__ void few_rows(const PagedArgs& a, const Part& w, char
       }
 #pragma unroll
       for (int db = 0; db < kDB; ++db) {
-        const i2v x = __builtin_amdgcn_ds_read_tr8_b64_v2i32((lds_i2v*)(uintptr_t)(((v_at + slot) ^ (db & 3) * 16) + (db >> 2) * 1024));
-        const h8 vf = __builtin_bit_cast(h8, from_e4m3<BF>(x[0], x[1], 1.f));
+        const h8 vf = __builtin_bit_cast(h8, from_e4m3<BF>(frag[db][0], frag[db][1], 1.f));
 #pragma unroll
         for (int cb = 0; cb < CB; ++cb) o[cb][db] = mma16<BF>(vf, __builtin_bit_cast(h8, pf[cb]), o[cb][db]);
       }
