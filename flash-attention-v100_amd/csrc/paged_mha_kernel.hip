@@ -205,6 +205,19 @@ struct Walk {
   }
   // Finds work group w's first item; false if it has none.
   __device__ __forceinline__ bool begin(const PagedArgs& a, int w, int lane) {
+    way = kWhole;
+    per_length = 0.f;
+    length = 1, round = 0, stretch = 0;
+    if (!a.shared && !a.ends) {  // as many items for each sequence: no need to look at others
+      const int each = paged_blocks(a.new_tokens * a.group, B::rows_of_block(a.new_tokens * a.group)) * a.kv_head;
+      items = each * a.batch;
+      if (w >= items) return false;
+      const int b = same(w / each);
+      load(a, b, lane);
+      upto = (long)(b + 1) * each;
+      x = w, end = items;
+      return true;
+    }
     load(a, 0, lane);
     long all = 0, count = 0;
     float heavy = 0.f, light = -INFINITY;  // light: less than 0, the least weight
@@ -212,15 +225,13 @@ struct Walk {
     for (int b = lane; b < a.batch; b += 64) {
       const Sequence s = one ? mine : sequence(a, b);
       const PagedLine t = weights(a, s.n, s.keys);
-      all += t.all() * a.kv_head;
       count += (long)t.blocks * a.kv_head;
+      if (!a.shared) continue;
+      all += t.all() * a.kv_head;
       heavy = fmaxf(heavy, heaviest(a, s.n, s.keys));
       if (s.n) light = fmaxf(light, -(float)t.of(0));
     }
     items = (int)of_lane(scan_over_wave(count), 63);
-    way = kWhole;
-    per_length = 0.f;
-    length = 1, round = 0, stretch = 0;
     if (a.shared) {
       all = of_lane(scan_over_wave(all), 63);
       heavy = same(max_over_wave(heavy));
