@@ -67,6 +67,15 @@ __device__ __forceinline__ PagedArgs args_again() {
   return a;
 }
 
+// A word of each 64 bytes of them, asked for at once: later loads find them in the scalar cache.
+__device__ __forceinline__ void touch_args() {
+  typedef __attribute__((address_space(4))) const unsigned Word;
+  Word* from = (Word*)__builtin_amdgcn_kernarg_segment_ptr();
+  static_assert(sizeof(PagedArgs) > 256 && sizeof(PagedArgs) <= 320, "five of them");
+  const unsigned w0 = from[0], w1 = from[16], w2 = from[32], w3 = from[48], w4 = from[64];
+  asm volatile("" ::"s"(w0), "s"(w1), "s"(w2), "s"(w3), "s"(w4));
+}
+
 struct Sequence {
   int first, n;  // its tokens
   int keys;
@@ -167,10 +176,18 @@ struct Part {
 };
 
 __device__ __forceinline__ float max_over_wave(float x) {
-#pragma unroll
-  for (int d = 1; d < 16; d *= 2) x = fmaxf(x, __shfl_xor(x, d));
+  auto turned = [](float y, auto by) __attribute__((always_inline)) {  // inside rows of 16 lanes
+    return __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(y), 0x120 + decltype(by)::value, 15, 15, true));
+  };
+  x = fmaxf(x, turned(x, IntTag<8>{}));
+  x = fmaxf(x, turned(x, IntTag<4>{}));
+  x = fmaxf(x, turned(x, IntTag<2>{}));
+  x = fmaxf(x, turned(x, IntTag<1>{}));
   return max_over_groups(x);
 }
+// A whole number below 2^62 as a float, and a quotient: nearly, and the same in all work groups.
+__device__ __forceinline__ float nearly(long x) { return fmaf((float)(unsigned)((unsigned long)x >> 32), 4294967296.f, (float)(unsigned)x); }
+__device__ __forceinline__ float nearly(float x, float y) { return x * __builtin_amdgcn_rcpf(y); }
 
 // A work group's items, one after the other (ways to share them: paged_plan.h); all lanes together, each with one of 64 sequences
 // in its registers.
@@ -229,7 +246,7 @@ struct Walk {
       if (!a.shared) continue;
       all += t.all() * a.kv_head;
       heavy = fmaxf(heavy, heaviest(a, s.n, s.keys));
-      if (s.n) light = fmaxf(light, -(float)t.of(0));
+      if (s.n) light = fmaxf(light, -nearly(t.of(0)));
     }
     items = (int)of_lane(scan_over_wave(count), 63);
     if (a.shared) {
@@ -238,16 +255,17 @@ struct Walk {
       const long even = paged_stretch(all);
       const int rounds = (items + kPagedGroups - 1) >> kPagedGroupsLog;
       light = -same(max_over_wave(light));
-      float best = rounds > 1 ? (float)rounds * ((float)all / (float)items)
+      float best = rounds > 1 ? (float)rounds * nearly(nearly(all), (float)items)
                               : fmaxf(B::kAlone * heavy, items <= kCus ? 0.f : 0.5f * (heavy + light));
-      if ((float)even + B::kStretchesCost < best) {
-        best = (float)even + B::kStretchesCost;
+      const float even_long = nearly(even);
+      if (even_long + B::kStretchesCost < best) {
+        best = even_long + B::kStretchesCost;
         way = kStretches;
         length = even;
       }
       if (one && items <= kPagedGroups) {
         // 64 lengths, from the even one up to five times that, by as many lanes: the best for which there are stretches enough
-        const float mine_long = (float)even * (1.f + lane * (1.f / 16.f)), mine_in = 1.f / mine_long;
+        const float mine_long = even_long * (1.f + lane * (1.f / 16.f)), mine_in = __builtin_amdgcn_rcpf(mine_long);
         const float weight = heaviest(a, mine.n, mine.keys);
         const int of_mine = weights(a, mine.n, mine.keys).blocks * a.kv_head;
         int parts = 0;
@@ -278,8 +296,8 @@ struct Walk {
     x = same(x);
     return x < end;
   }
+  __device__ __forceinline__ bool more() const { return x < end; }
   __device__ __forceinline__ bool next(const PagedArgs& a, int lane, Part& r) {
-    if (x >= end) return false;
     unsigned long long past;
     while (!(past = __builtin_amdgcn_ballot_w64(upto > x))) {
       if (b0 + 64 >= a.batch) return false;
@@ -725,7 +743,7 @@ __device__ __forceinline__ void few_rows(const PagedArgs& a, const Part& w, char
     const float sum = over_groups_sum(l[cb]);
     if (g == 0) join[wave][16 * cb + m] = float2{mc[cb], bad ? NAN : sum};
   }
-  __syncthreads();
+  block_barrier();
   float* const mine = reinterpret_cast<float*>(smem + wave * G::kWaveBytes);
 #pragma unroll
   for (int cb = 0; cb < CB; ++cb) {
@@ -737,7 +755,7 @@ __device__ __forceinline__ void few_rows(const PagedArgs& a, const Part& w, char
     for (int db = 0; db < kDB; ++db)
       *reinterpret_cast<f4v*>(reinterpret_cast<char*>(mine) + (16 * cb + m) * G::kPitch + db * 64 + g * 16) = o[cb][db] * f;
   }
-  __syncthreads();
+  block_barrier();
   constexpr int kPieces = D / 4;  // of a row
   for (int i = threadIdx.x; i < kRows * kPieces; i += kFewWaves * 64) {
     const int row = i / kPieces, piece = i % kPieces;
@@ -1306,6 +1324,7 @@ __global__ void __launch_bounds__(kPagedThreads, 2) paged_forward_kernel(PagedAr
     for (long i = from + ((long)blockIdx.x * blockDim.x + threadIdx.x) * 16; i < to; i += (long)gridDim.x * blockDim.x * 16)
       *reinterpret_cast<u4v*>(a.o + i) = u4v{0, 0, 0, 0};
   }
+  touch_args();
   const int lane = threadIdx.x & 63;
   Walk<B> walk;
   if (!walk.begin(a, blockIdx.x, lane)) return;
@@ -1318,7 +1337,8 @@ __global__ void __launch_bounds__(kPagedThreads, 2) paged_forward_kernel(PagedAr
     } else {
       if constexpr (FEW != 0) few_rows<D, FEW / 16, BF, Q8>(a, w, smem, B::kMost);
     }
-    __syncthreads();  // the next item takes the same LDS
+    if (!walk.more()) return;
+    block_barrier();  // the next item takes the same LDS
   }
 }
 
