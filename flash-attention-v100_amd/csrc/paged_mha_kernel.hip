@@ -136,13 +136,22 @@ __device__ __forceinline__ long moved(long x) {
   const unsigned hi = __builtin_amdgcn_update_dpp(0, (int)((unsigned long)x >> 32), kMove, kRows, 15, false);
   return (long)(((unsigned long)hi << 32) | lo);
 }
+__device__ __forceinline__ int scan_over_wave(int x) {
+  x += __builtin_amdgcn_update_dpp(0, x, 0x111, 15, 15, false);
+  x += __builtin_amdgcn_update_dpp(0, x, 0x112, 15, 15, false);
+  x += __builtin_amdgcn_update_dpp(0, x, 0x114, 15, 15, false);
+  x += __builtin_amdgcn_update_dpp(0, x, 0x118, 15, 15, false);
+  x += __builtin_amdgcn_update_dpp(0, x, 0x142, 10, 15, false);  // lane 15 of rows 0 and 2 to rows 1 and 3
+  x += __builtin_amdgcn_update_dpp(0, x, 0x143, 12, 15, false);  // lane 31 to rows 2 and 3
+  return x;
+}
 __device__ __forceinline__ long scan_over_wave(long x) {
   x += moved<0x111, 15>(x);
   x += moved<0x112, 15>(x);
   x += moved<0x114, 15>(x);
   x += moved<0x118, 15>(x);
-  x += moved<0x142, 10>(x);  // lane 15 of rows 0 and 2 to rows 1 and 3
-  x += moved<0x143, 12>(x);  // lane 31 to rows 2 and 3
+  x += moved<0x142, 10>(x);
+  x += moved<0x143, 12>(x);
   return x;
 }
 
@@ -154,6 +163,7 @@ struct Blocks {
   static constexpr int kMost = MANY ? kManyRows : FEW;  // rows of a slot
   static __device__ __forceinline__ bool many(int rows) { return MANY && (FEW == 0 || rows > kFewRows); }
   static __device__ __forceinline__ int rows_of_block(int rows) { return many(rows) ? kManyRows : FEW; }
+  static __device__ __forceinline__ int count(int rows) { return paged_blocks(rows, rows_of_block(rows)); }
   // What an item costs beside its keys, in keys: about three tiles where a block has many rows, one where it has few.
   static __device__ __forceinline__ int overhead(int rows) { return many(rows) ? 192 : 64; }
   // Weight of a key: 4 for a block of many rows while another shares its CU.  Beside such blocks those of few rows, which wait for
@@ -190,17 +200,21 @@ __device__ __forceinline__ float nearly(long x) { return fmaf((float)(unsigned)(
 __device__ __forceinline__ float nearly(float x, float y) { return x * __builtin_amdgcn_rcpf(y); }
 
 // A work group's items, one after the other (ways to share them: paged_plan.h); all lanes together, each with one of 64 sequences
-// in its registers.
+// in its registers.  Every work group finds its own from the lengths of all sequences; what it takes for that is time during which
+// no memory is read, so whole numbers of 32 bits serve wherever they can.
 template <typename B>
 struct Walk {
   enum Way { kStretches, kParts, kWhole };
-  long x, end, length;  // position; end of the stretch and its length
-  long upto;            // the line up to the end of the lane's sequence
-  int stretch, b0;      // b0: the first of the 64 sequences
-  int round, items;     // of kWhole
-  float per_length;     // of kParts: for paged_parts
   Way way;
+  int b0;  // the first of the 64 sequences
   Sequence mine;
+  // kParts and kWhole, where an item has `parts` places in a line of them
+  int at, items, round;
+  int upto, parts;  // the line up to the end of the lane's sequence; of an item of the lane's sequence
+  // kStretches
+  long x, end, length;  // position; end of the stretch and its length
+  long line_upto;
+  int stretch;
   __device__ __forceinline__ static PagedLine weights(const PagedArgs& a, int n, int keys) {
     const int rows = n * a.group;
     return paged_line(keys, n, a.group, a.causal ? a.step[B::many(rows)] : 0, B::rows_of_block(rows), B::overhead(rows), B::of_key(rows));
@@ -209,101 +223,106 @@ struct Walk {
     const int rows = n * a.group;
     return n == 0 ? 0.f : (float)(B::of_key(rows) * (keys + B::overhead(rows)));
   }
-  __device__ __forceinline__ PagedLine line(const PagedArgs& a, int n, int keys) const {
-    if (way == kStretches) return weights(a, n, keys);
-    return paged_line_of_parts(way == kWhole ? 1 : paged_parts(heaviest(a, n, keys), per_length), n, a.group, B::rows_of_block(n * a.group));
-  }
-  __device__ __forceinline__ void scan(const PagedArgs& a, long before, int lane) {
-    upto = before + scan_over_wave(b0 + lane < a.batch ? line(a, mine.n, mine.keys).all() * a.kv_head : 0);
-  }
   __device__ __forceinline__ void load(const PagedArgs& a, int from, int lane) {
     b0 = from;
     mine = sequence(a, min(b0 + lane, a.batch - 1));
   }
+  __device__ __forceinline__ void scan(const PagedArgs& a, int before, int lane) {  // not of kStretches
+    upto = before + scan_over_wave(b0 + lane < a.batch ? B::count(mine.n * a.group) * (int)a.kv_head * parts : 0);
+  }
+  __device__ __forceinline__ void scan(const PagedArgs& a, long before, int lane) {
+    line_upto = before + scan_over_wave(b0 + lane < a.batch ? weights(a, mine.n, mine.keys).all() * a.kv_head : 0);
+  }
   // Finds work group w's first item; false if it has none.
   __device__ __forceinline__ bool begin(const PagedArgs& a, int w, int lane) {
     way = kWhole;
-    per_length = 0.f;
-    length = 1, round = 0, stretch = 0;
+    parts = 1, round = 0, stretch = 0;
+    x = end = length = line_upto = 0;
     if (!a.shared && !a.ends) {  // as many items for each sequence: no need to look at others
-      const int each = paged_blocks(a.new_tokens * a.group, B::rows_of_block(a.new_tokens * a.group)) * a.kv_head;
+      const int each = B::count(a.new_tokens * a.group) * a.kv_head;
       items = each * a.batch;
       if (w >= items) return false;
       const int b = same(w / each);
       load(a, b, lane);
-      upto = (long)(b + 1) * each;
-      x = w, end = items;
+      upto = (b + 1) * each;
+      at = w;
       return true;
     }
     load(a, 0, lane);
-    long all = 0, count = 0;
-    float heavy = 0.f, light = -INFINITY;  // light: less than 0, the least weight
     const bool one = a.batch <= 64;
+    scan(a, 0, lane);
+    items = __builtin_amdgcn_readlane(upto, 63);
+    if (!one) {
+      int more = 0;
+      for (int b = 64 + lane; b < a.batch; b += 64) more += B::count(sequence(a, b).n * a.group) * (int)a.kv_head;
+      items += __builtin_amdgcn_readlane(scan_over_wave(more), 63);
+    }
+    if (!a.shared) {
+      at = w;
+      return at < items;
+    }
+    long all = 0;
+    float heavy = 0.f, light = -INFINITY;  // light: less than 0, the least weight
     for (int b = lane; b < a.batch; b += 64) {
       const Sequence s = one ? mine : sequence(a, b);
       const PagedLine t = weights(a, s.n, s.keys);
-      count += (long)t.blocks * a.kv_head;
-      if (!a.shared) continue;
       all += t.all() * a.kv_head;
       heavy = fmaxf(heavy, heaviest(a, s.n, s.keys));
       if (s.n) light = fmaxf(light, -nearly(t.of(0)));
     }
-    items = (int)of_lane(scan_over_wave(count), 63);
-    if (a.shared) {
-      all = of_lane(scan_over_wave(all), 63);
-      heavy = same(max_over_wave(heavy));
-      const long even = paged_stretch(all);
-      const int rounds = (items + kPagedGroups - 1) >> kPagedGroupsLog;
-      light = -same(max_over_wave(light));
-      float best = rounds > 1 ? (float)rounds * nearly(nearly(all), (float)items)
-                              : fmaxf(B::kAlone * heavy, items <= kCus ? 0.f : 0.5f * (heavy + light));
-      const float even_long = nearly(even);
-      if (even_long + B::kStretchesCost < best) {
-        best = even_long + B::kStretchesCost;
-        way = kStretches;
-        length = even;
-      }
-      if (one && items <= kPagedGroups) {
-        // 64 lengths, from the even one up to five times that, by as many lanes: the best for which there are stretches enough
-        const float mine_long = even_long * (1.f + lane * (1.f / 16.f)), mine_in = __builtin_amdgcn_rcpf(mine_long);
-        const float weight = heaviest(a, mine.n, mine.keys);
-        const int of_mine = weights(a, mine.n, mine.keys).blocks * a.kv_head;
-        int parts = 0;
-        for (int b = 0; b < a.batch; ++b)
-          parts += __builtin_amdgcn_readlane(of_mine, b) * paged_parts(__uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(weight), b)), mine_in);
-        const float cost = parts <= kCus ? B::kAlone * mine_long + 0.5f * B::kPartsCost : parts <= kPagedGroups ? mine_long + B::kPartsCost : INFINITY;
-        const float least = -same(max_over_wave(-cost));
-        if (least < best) {
-          const int l = __builtin_ctzll(__builtin_amdgcn_ballot_w64(cost == least));
-          way = kParts;
-          per_length = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(mine_in), l));
-          all = __builtin_amdgcn_readlane(parts, l);
-          length = 1;
-        }
+    all = of_lane(scan_over_wave(all), 63);
+    heavy = same(max_over_wave(heavy));
+    light = -same(max_over_wave(light));
+    const long even = paged_stretch(all);
+    const float even_long = nearly(even);
+    const int rounds = (items + kPagedGroups - 1) >> kPagedGroupsLog;
+    float best = rounds > 1 ? (float)rounds * nearly(nearly(all), (float)items)
+                            : fmaxf(B::kAlone * heavy, items <= kCus ? 0.f : 0.5f * (heavy + light));
+    if (even_long + B::kStretchesCost < best) {
+      best = even_long + B::kStretchesCost;
+      way = kStretches;
+    }
+    int places = 0;
+    if (one && items <= kPagedGroups) {
+      // 64 lengths, from the even one up to five times that, by as many lanes: the best for which there are stretches enough
+      const float mine_long = even_long * (1.f + lane * (1.f / 16.f)), mine_in = __builtin_amdgcn_rcpf(mine_long);
+      const float weight = heaviest(a, mine.n, mine.keys);
+      const int of_mine = B::count(mine.n * a.group) * (int)a.kv_head;
+      int count = 0;
+      for (int b = 0; b < a.batch; ++b)
+        count += __builtin_amdgcn_readlane(of_mine, b) * paged_parts(__uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(weight), b)), mine_in);
+      const float cost = count <= kCus ? B::kAlone * mine_long + 0.5f * B::kPartsCost : count <= kPagedGroups ? mine_long + B::kPartsCost : INFINITY;
+      const float least = -same(max_over_wave(-cost));
+      if (least < best) {
+        const int l = __builtin_ctzll(__builtin_amdgcn_ballot_w64(cost == least));
+        way = kParts;
+        places = __builtin_amdgcn_readlane(count, l);
+        parts = paged_parts(weight, __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(mine_in), l)));
+        scan(a, 0, lane);
       }
     }
     way = (Way)same((int)way);
-    length = same(length);
-    scan(a, 0, lane);
-    if (way == kWhole) {
-      x = a.shared ? paged_whole(0, w, items) : w;
-      end = items;
-    } else {
-      stretch = same(paged_spread(w, way == kParts ? (int)all : paged_stretches(all, length)));
-      x = stretch * length;
+    if (way == kStretches) {
+      scan(a, 0l, lane);
+      length = same(even);
+      stretch = same(paged_spread(w, paged_stretches(all, length)));
+      x = same(stretch * length);
       end = same(min(x + length, all));
+      return x < end;
     }
-    x = same(x);
-    return x < end;
+    at = same(way == kParts ? paged_spread(w, places) : paged_whole(0, w, items));
+    return at < (way == kParts ? places : items);
   }
-  __device__ __forceinline__ bool more() const { return x < end; }
+  __device__ __forceinline__ bool more() const { return way == kStretches ? x < end : way == kWhole && at < items; }
   __device__ __forceinline__ bool next(const PagedArgs& a, int lane, Part& r) {
     unsigned long long past;
-    while (!(past = __builtin_amdgcn_ballot_w64(upto > x))) {
+    while (!(past = __builtin_amdgcn_ballot_w64(way == kStretches ? line_upto > x : upto > at))) {
       if (b0 + 64 >= a.batch) return false;
-      const long before = of_lane(upto, 63);
+      const long line_before = of_lane(line_upto, 63);
+      const int before = __builtin_amdgcn_readlane(upto, 63);
       load(a, b0 + 64, lane);
-      scan(a, before, lane);
+      if (way == kStretches) scan(a, line_before, lane);
+      else scan(a, before, lane);
     }
     const int l = __builtin_ctzll(past);
     r.b = b0 + l;
@@ -311,39 +330,51 @@ struct Walk {
     r.s.n = __builtin_amdgcn_readlane(mine.n, l);
     r.s.keys = __builtin_amdgcn_readlane(mine.keys, l);
     r.s.past = __builtin_amdgcn_readlane(mine.past, l);
-    const PagedLine heads = line(a, r.s.n, r.s.keys);
-    const long of_head = heads.all(), base = of_lane(upto, l) - of_head * a.kv_head;
-    long item = 0, weight = 1;
-    if (way == kWhole) {
-      paged_whole_item((int)(x - base), heads.blocks, a.kv_head, r.block, r.head);
+    const int rows = r.s.n * a.group, blocks = B::count(rows);
+    if (way != kStretches) {
+      const int each = __builtin_amdgcn_readlane(parts, l), of_head = blocks * each;
+      const int local = at - (__builtin_amdgcn_readlane(upto, l) - of_head * (int)a.kv_head);
+      int part = 0;
+      if (way == kWhole) {
+        paged_whole_item(local, blocks, a.kv_head, r.block, r.head);
+      } else {
+        r.head = same(paged_divide(local, of_head));
+        r.block = same(paged_divide(local - r.head * of_head, each));
+        part = local - r.head * of_head - r.block * each;
+      }
       r.block = same(r.block), r.head = same(r.head);
-    } else {
-      r.head = same(paged_divide(x - base, of_head));
-      const long from = base + r.head * of_head;
-      r.block = heads.blocks == 1 ? 0 : same(paged_block_at(heads, x - from));
-      item = from + heads.before(r.block), weight = heads.of(r.block);
+      const int tiles = tiles_of(a, r, rows);
+      const float per = (float)tiles * __builtin_amdgcn_rcpf((float)each);  // the same in all parts
+      r.t0 = part == 0 ? 0 : same((int)((float)part * per));
+      r.t1 = part + 1 == each ? tiles : same((int)((float)(part + 1) * per));
+      r.opens = part == 0;
+      r.whole = each == 1;
+      r.parts = each;
+      r.place = paged_place(at - part, part);
+      r.stretch = at;
+      at = way == kWhole && a.shared ? same(paged_whole(++round, blockIdx.x, items)) : items;
+      return true;
     }
-    const int rows = r.s.n * a.group, last = min(rows, (r.block + 1) * B::rows_of_block(rows)) - 1;
-    const int tiles = paged_tiles(paged_visible(r.s.keys, r.s.n, last / a.group, a.causal));
+    const PagedLine heads = weights(a, r.s.n, r.s.keys);
+    const long of_head = heads.all(), base = of_lane(line_upto, l) - of_head * a.kv_head;
+    r.head = same(paged_divide(x - base, of_head));
+    const long from = base + r.head * of_head;
+    r.block = blocks == 1 ? 0 : same(paged_block_at(heads, x - from));
+    const long item = from + heads.before(r.block), weight = heads.of(r.block);
+    const int tiles = tiles_of(a, r, rows);
+    r.t0 = same(paged_tile_at(tiles, x - item, weight));
+    r.t1 = same(paged_tile_at(tiles, end - item, weight));
+    r.opens = same((int)(item >= x));
+    r.whole = r.opens && same((int)(item + weight <= end));
+    r.parts = r.whole || !r.opens ? 1 : same(paged_divide(item + weight - 1, length)) - stretch + 1;
+    r.place = paged_place(stretch, r.opens ? 0 : 1) - (r.opens ? 0 : 2);
     r.stretch = stretch;
-    if (way == kWhole) {
-      r.t0 = 0, r.t1 = tiles;
-      r.opens = r.whole = true;
-      r.parts = 1, r.place = 0;
-      x = a.shared ? paged_whole(++round, blockIdx.x, items) : end;
-    } else {
-      r.t0 = paged_tile_at(tiles, x - item, weight);
-      r.t1 = paged_tile_at(tiles, end - item, weight);
-      r.opens = item >= x;
-      r.whole = r.opens && item + weight <= end;
-      r.parts = r.whole || !r.opens ? 1 : paged_divide(item + weight - 1, length) - stretch + 1;
-      r.place = paged_place(stretch, r.opens ? 0 : 1) - (r.opens ? 0 : 2);
-      x = item + weight;
-    }
-    x = same(x);
-    r.t0 = same(r.t0), r.t1 = same(r.t1), r.parts = same(r.parts), r.place = same(r.place);
-    r.opens = same((int)r.opens), r.whole = same((int)r.whole);
+    x = same(item + weight);
     return true;
+  }
+  __device__ __forceinline__ static int tiles_of(const PagedArgs& a, const Part& r, int rows) {
+    const int last = min(rows, (r.block + 1) * B::rows_of_block(rows)) - 1;
+    return paged_tiles(paged_visible(r.s.keys, r.s.n, last / a.group, a.causal));
   }
 };
 

@@ -42,16 +42,12 @@ FMHA_HOST_DEVICE PagedLine paged_line(int keys, int new_tokens, const Int& group
   const int hidden = step == 0 ? 0 : new_tokens < keys ? new_tokens : keys;
   return PagedLine{of_key * (long)(keys - hidden + overhead), step, paged_blocks(new_tokens * group, rows_of_block)};
 }
-// In stretches, where every item has a whole number of them.
-template <typename Int>
-FMHA_HOST_DEVICE PagedLine paged_line_of_parts(int parts, int new_tokens, const Int& group, int rows_of_block) {
-  return PagedLine{parts, 0, paged_blocks(new_tokens * group, rows_of_block)};
-}
 // Parts of an item of that weight, none of them longer than 1 / per_length.
 FMHA_HOST_DEVICE int paged_parts(float weight, float per_length) { return (int)(weight * per_length) + 1; }
 
 // n / d where that is below 2^20: by floats, put right.
-FMHA_HOST_DEVICE int paged_divide(long n, long d) {
+template <typename Int>  // int or long
+FMHA_HOST_DEVICE int paged_divide(Int n, Int d) {
   int q = (int)((float)n / (float)d);
   if (q * d > n) --q;
   if ((q + 1) * d <= n) ++q;

@@ -270,18 +270,18 @@ int main() {
   auto rnd = [&](int n) { seed = seed * 1664525u + 1013904223u; return (int)((seed >> 8) % (unsigned)n); };
   for (int round = 0; round < 3000; ++round) {
     const int batch = 1 + rnd(12), kv = 1 + rnd(4), group = 1 + rnd(9), rows_of_block = rnd(2) ? 32 : 128;
-    const bool causal = rnd(2), ones = rnd(8) == 0;
+    const bool causal = rnd(2);
     std::vector<Seq> seqs(batch);
     std::vector<PagedLine> lines(batch);
     long all = 0;
     for (int b = 0; b < batch; ++b) {
       seqs[b] = {rnd(3) ? rnd(3) : rnd(300), rnd(3) ? rnd(500) : rnd(20000)};
-      lines[b] = ones ? paged_line_of_parts(1 + rnd(5), seqs[b].n, group, rows_of_block) : paged_line(seqs[b].keys, seqs[b].n, group, causal ? paged_step(rows_of_block, group, 4) : 0, rows_of_block, 64, 4);
+      lines[b] = paged_line(seqs[b].keys, seqs[b].n, group, causal ? paged_step(rows_of_block, group, 4) : 0, rows_of_block, 64, 4);
       all += lines[b].all() * kv;
     }
-    const long length = ones ? 1 : paged_stretch(all);
-    const int stretches = ones ? (int)all : paged_stretches(all, length);
-    if (stretches * length < all || (!ones && stretches > kPagedGroups)) return puts("stretches"), 1;
+    const long length = paged_stretch(all);
+    const int stretches = paged_stretches(all, length);
+    if (stretches * length < all || stretches > kPagedGroups) return puts("stretches"), 1;
     struct Item { int next = 0, tiles = -1, parts = 0, told = 0, first = 0; };
     std::map<std::vector<int>, Item> items;
     std::map<int, int> places;
@@ -320,7 +320,7 @@ int main() {
       for (int h = 0; h < kv; ++h)
         for (int k = 0; k < lines[b].blocks; ++k) {
           const Item it = items[{b, h, k}];
-          if (it.next != it.tiles || it.parts != it.told || (ones && it.parts != lines[b].first)) return puts("not whole"), 1;
+          if (it.next != it.tiles || it.parts != it.told) return puts("not whole"), 1;
         }
   }
   puts("ok");
@@ -337,6 +337,8 @@ int main() {
   for (int i = 0; i < 4000000; ++i) {
     const long d = rnd(1 + i % 41) + 1, n = d * rnd(1 + i % 20) + rnd(1 + i % 41) % d;
     if (paged_divide(n, d) != n / d || paged_divide(n / d * d, d) != n / d) return puts("wrong"), 1;
+    const int m = (int)(rnd(30)), e = (int)(rnd(20)) + 1 + m / (1 << 20);
+    if (paged_divide(m, e) != m / e) return puts("wrong int"), 1;
   }
   puts("ok");
 }
