@@ -1473,7 +1473,7 @@ struct WriteArgs {
   CacheStrides ks, vs, kss, vss;
   const int *table, *keys, *ends;
   long table_stride;
-  int batch, new_tokens, tokens, kv_head, pages, width;
+  int batch, tokens, kv_head, pages, width;
   FmhaDivisor page_size, per_sequence;  // per_sequence: new tokens of each, where ends is null
 };
 
@@ -1558,7 +1558,7 @@ struct ReadArgs {
   int max_seqlen, pages, width;
   FmhaDivisor page_size, kv_head, blocks;  // blocks: work groups of a sequence
 };
-constexpr int kReadSteps = 8;
+constexpr int kReadSteps = 4;  // all of whose page numbers are asked for, then all rows
 
 template <int D, bool BF, bool Q8>
 __global__ void __launch_bounds__(256) paged_read_kernel(ReadArgs a) {
@@ -1570,30 +1570,40 @@ __global__ void __launch_bounds__(256) paged_read_kernel(ReadArgs a) {
   const unsigned char* const scales = value ? a.v_scale : a.k_scale;
   const CacheStrides st = value ? a.vs : a.ks, sst = value ? a.vss : a.kss;
   char* const out = (value ? a.v : a.k) + (long)b * a.max_seqlen * (int)a.kv_head * D * 2;
-  const int row0 = block * (256 * kReadSteps / kChunks);
+  const int row0 = block * (256 * kReadSteps / kChunks) + threadIdx.x / kChunks, chunk = threadIdx.x % kChunks;
+  const int* const table = a.table + b * a.table_stride;
+  int pos[kReadSteps], head[kReadSteps], slot[kReadSteps], id[kReadSteps];
 #pragma unroll
   for (int u = 0; u < kReadSteps; ++u) {
-    const int row = row0 + (u * 256 + threadIdx.x) / kChunks, chunk = threadIdx.x % kChunks;
-    const int pos = row / a.kv_head, head = row - pos * (int)a.kv_head;
-    if (pos >= a.max_seqlen) continue;
-    u4v x = {0, 0, 0, 0};
-    if (pos < keys) {
-      const int page_at = pos / a.page_size, slot = pos - page_at * (int)a.page_size;
-      const long id = page_at < a.width ? a.table[b * a.table_stride + page_at] : -1;
-      if (id < 0 || id >= a.pages) {
-        x[0] = x[1] = x[2] = x[3] = BF ? 0x7fc07fc0u : 0x7e007e00u;  // NaN
-      } else {
-        const char* const from = cache + id * st.page + (long)slot * st.slot + (long)head * st.head;
-        if constexpr (Q8) {
-          const u2v y = *reinterpret_cast<const u2v*>(from + chunk * 8);
-          const unsigned s = scales[id * sst.page + (long)slot * sst.slot + (long)head * sst.head];
-          x = from_e4m3<BF>(y[0], y[1], scale_of(s));
-        } else {
-          x = *reinterpret_cast<const u4v*>(from + chunk * 16);
-        }
-      }
+    const int row = row0 + u * (256 / kChunks);
+    pos[u] = row / a.kv_head, head[u] = row - pos[u] * (int)a.kv_head;
+    const int page_at = pos[u] / a.page_size;
+    slot[u] = pos[u] - page_at * (int)a.page_size;
+    id[u] = page_at < a.width ? table[page_at] : -1;
+  }
+  u4v x[kReadSteps];
+#pragma unroll
+  for (int u = 0; u < kReadSteps; ++u) {
+    x[u] = u4v{0, 0, 0, 0};
+    if (pos[u] >= min(keys, a.max_seqlen)) continue;
+    if (id[u] < 0 || id[u] >= a.pages) {
+      x[u] = BF ? u4v{0x7fc07fc0u, 0x7fc07fc0u, 0x7fc07fc0u, 0x7fc07fc0u} : u4v{0x7e007e00u, 0x7e007e00u, 0x7e007e00u, 0x7e007e00u};  // NaN
+      continue;
     }
-    *reinterpret_cast<u4v*>(out + (long)row * (D * 2) + chunk * 16) = x;
+    const char* const from = cache + id[u] * st.page + (long)slot[u] * st.slot + (long)head[u] * st.head;
+    if constexpr (Q8) {
+      const u2v y = *reinterpret_cast<const u2v*>(from + chunk * 8);
+      const unsigned s = scales[id[u] * sst.page + (long)slot[u] * sst.slot + (long)head[u] * sst.head];
+      x[u] = u4v{y[0], y[1], s, 1};
+    } else {
+      x[u] = *reinterpret_cast<const u4v*>(from + chunk * 16);
+    }
+  }
+#pragma unroll
+  for (int u = 0; u < kReadSteps; ++u) {
+    if (pos[u] >= a.max_seqlen) continue;
+    if (Q8 && x[u][3] == 1) x[u] = from_e4m3<BF>(x[u][0], x[u][1], scale_of(x[u][2]));  // neither zeros nor NaN end in 1
+    *reinterpret_cast<u4v*>(out + (long)(row0 + u * (256 / kChunks)) * (D * 2) + chunk * 16) = x[u];
   }
 }
 
