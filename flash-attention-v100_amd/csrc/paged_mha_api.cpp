@@ -49,6 +49,11 @@ void check_no_grad(std::initializer_list<const at::Tensor*> xs) {
   TORCH_CHECK(!torch::jit::tracer::isTracing(), "the paged cache is not supported under torch.jit.trace");
 }
 
+// For autograd, which holds tensors that were saved before.
+void written(const at::Tensor& x) {
+  if (!x.is_inference()) x.unsafeGetTensorImpl()->bump_version();
+}
+
 paged_mha_strides cache_strides(const at::Tensor& x) { return {x.stride(0), x.stride(1), x.stride(2)}; }
 
 // Cache and batch as the C interface takes them.
@@ -164,6 +169,7 @@ at::Tensor paged_attention(const at::Tensor& q, const at::Tensor& k_cache, const
                                 is_causal ? 1 : 0, out_.has_value() ? 0 : 1, bytes ? workspace.data_ptr() : nullptr, bytes,
                                 c10::hip::getCurrentHIPStream().stream()),
               "paged_mha_forward");
+  if (out_.has_value()) written(out);
   return out;
 }
 
@@ -175,11 +181,16 @@ void cache_write(const at::Tensor& k, const at::Tensor& v, const at::Tensor& k_c
   p.set_tokens(k, "key", p.cache.kv_head);
   p.set_tokens(v, "value", p.cache.kv_head);
   TORCH_CHECK(k.sizes() == v.sizes(), "key and value must have the same shape");
-  at::assert_no_internal_overlap(k_cache);
-  at::assert_no_internal_overlap(v_cache);
+  at::assert_no_overlap(k_cache, v_cache);
+  for (const at::Tensor* x : {&k_cache, &v_cache}) {
+    at::assert_no_internal_overlap(*x);
+    at::assert_no_overlap(*x, k);
+    at::assert_no_overlap(*x, v);
+  }
   if (k_scale.has_value()) {
     at::assert_no_internal_overlap(*k_scale);
     at::assert_no_internal_overlap(*v_scale);
+    at::assert_no_overlap(*k_scale, *v_scale);
   }
   check_devices(k_cache, {&k, &v, &v_cache, &page_table, &cache_seqlens}, {&cu_seqlens, &k_scale, &v_scale});
   const api::OnDeviceOf device_guard(k_cache);
@@ -187,6 +198,8 @@ void cache_write(const at::Tensor& k, const at::Tensor& v, const at::Tensor& k_c
   check_paged(paged_mha_write(&p.cache, &p.batch, ko.x.data_ptr(), &ko.st, vo.x.data_ptr(), &vo.st,
                               c10::hip::getCurrentHIPStream().stream()),
               "paged_mha_write");
+  written(k_cache), written(v_cache);
+  if (k_scale.has_value()) written(*k_scale), written(*v_scale);
 }
 
 std::tuple<at::Tensor, at::Tensor> cache_read(const at::Tensor& k_cache, const at::Tensor& v_cache, const at::Tensor& page_table,

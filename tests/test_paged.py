@@ -385,3 +385,33 @@ def test_outputs_that_overlap_inputs_are_refused(ops):
     batch = paged.Batch([40], 1, 2, 2)
     with pytest.raises(RuntimeError, match="memory"):
         ops.flash_attn_paged_func(batch.q, *batch.args(), out=batch.q)
+
+
+def test_caches_that_overlap_are_refused(ops):
+    batch = paged.Batch([40], 1, 2, 1)
+    _, v_cache, *rest = batch.args()
+    with pytest.raises(RuntimeError, match="memory"):
+        ops.kv_cache_write(batch.k, batch.v, v_cache, v_cache, *rest)
+    row = v_cache[:1, :1]  # of a token, as k of one
+    with pytest.raises(RuntimeError, match="memory"):
+        ops.kv_cache_write(row, batch.v, *batch.args())
+    batch = paged.Batch([40], 1, 2, 1, cache="e4m3")
+    with pytest.raises(RuntimeError, match="memory"):
+        ops.kv_cache_write(batch.k, batch.v, *batch.args(), k_scale=batch.v_scale, v_scale=batch.v_scale)
+
+
+def test_written_tensors_count_as_changed(ops):
+    """A graph that saved one of them must not use it afterwards."""
+    batch = paged.Batch([40], 1, cache="e4m3")
+    tensors = [batch.k_cache, batch.v_cache, batch.k_scale, batch.v_scale]
+    before = [x._version for x in tensors]
+    ops.kv_cache_write(batch.k, batch.v, *batch.args(), **batch.scales())
+    assert all(x._version > n for x, n in zip(tensors, before))
+    out = torch.empty_like(batch.q)
+    leaf = torch.ones_like(out, requires_grad=True)
+    product = (leaf * out).sum()
+    ops.flash_attn_paged_func(batch.q, *batch.args(), out=out, **batch.scales())
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        product.backward()
+    with torch.inference_mode():  # tensors without a version
+        ops.flash_attn_paged_func(batch.q, *batch.args(), out=torch.empty_like(batch.q), **batch.scales())
