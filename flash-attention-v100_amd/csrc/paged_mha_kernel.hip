@@ -221,7 +221,7 @@ struct Walk {
   }
   __device__ __forceinline__ static float heaviest(const PagedArgs& a, int n, int keys) {
     const int rows = n * a.group;
-    return n == 0 ? 0.f : (float)(B::of_key(rows) * (keys + B::overhead(rows)));
+    return n == 0 ? 0.f : (float)B::of_key(rows) * (float)(keys + B::overhead(rows));  // past 32 bits
   }
   __device__ __forceinline__ void load(const PagedArgs& a, int from, int lane) {
     b0 = from;
@@ -1418,7 +1418,6 @@ __global__ void __launch_bounds__(256) paged_join_kernel(PagedArgs a, int slot_r
   constexpr int kPieces = D / 4, kSlices = 256 / kPieces;
   __shared__ Joined sums[kSlices][kPieces];
   const int slice = threadIdx.x / kPieces, piece = threadIdx.x % kPieces, rows = a.tokens * a.head;
-  const long room = 2l * kPagedGroups * slot_rows;
   auto place = [&](int row) __attribute__((always_inline)) {
     if (row >= rows) return int2{0, 1};
     if (a.ends) {
@@ -1427,7 +1426,7 @@ __global__ void __launch_bounds__(256) paged_join_kernel(PagedArgs a, int slot_r
     }
     int2 r = a.places[row];
     // of tokens that ranges which make no sense left out it says anything
-    if (r.x < 0 || r.y < 1 || r.x + (2l * r.y + 1) * slot_rows > room) r.y = 1;
+    if (!paged_parts_fit(r.x, r.y, slot_rows)) r.y = 1;
     return r;
   };
   auto store = [&](int row, const Joined& r) __attribute__((always_inline)) {
@@ -1658,7 +1657,13 @@ struct Launch {
   bool shared;
   int place_rows() const { return many ? kManyRows : few; }
   long grid() const { return shared ? kPagedGroups : (items + 7) / 8 * 8; }
+  // Rows that a work group of the second launch looks at: one where most of them have parts, more where few do, as only
+  // 2 * kPagedGroups blocks can have any.  Both launches for single tokens of 1000 keys, 32 heads of 128, one row and 32 of them:
+  // 160 sequences 106.9 us and 106.5, 256 164.9 and 161.5, 512 312.6 and 305.0, 1024 616 and 601.
+  int join_rows(long rows) const { return many || rows > 4096 ? 32 : 1; }
+  long join_grid(long rows) const { return (rows + join_rows(rows) - 1) / join_rows(rows); }
 };
+constexpr long kMostGroups = (1l << 32) / 256 - 1;  // a launch has fewer than 2^32 work items
 // The bits below which all offsets of 16 positions are 0, and whether the bits above fit 32.
 bool fits(const paged_mha_cache* c, const paged_mha_strides& s, int bytes, int& shift) {
   const unsigned long long page = s.page * bytes, slot = s.slot * bytes * 16, any = page | slot;
@@ -1679,7 +1684,8 @@ Launch plan(const paged_mha_cache* c, const paged_mha_batch* b, int head, int ma
   const int least_rows = p.few ? p.few : kManyRows;
   const long blocks = b->cu_seqlens ? b->tokens * group / least_rows + b->batch : b->batch * ((b->tokens * group + least_rows - 1) / least_rows);
   p.items = blocks * c->kv_head;
-  p.shared = (long)b->table_width * c->page_size * 4 > kPagedLeast;
+  // Items of up to 256 keys are not split: a work group each, unless each would look through a long batch for its own.
+  p.shared = (long)b->table_width * c->page_size * 4 > kPagedLeast || (b->cu_seqlens && b->batch > 64);
   return p;
 }
 // Sums of the parts' rows, their maxima and totals, where each row of o has its parts.
@@ -1691,8 +1697,8 @@ template <int D, int FEW, bool MANY, bool BF, bool Q8>
 int launch_forward(const Launch& p, const PagedArgs& a, hipStream_t stream) {
   if (launch(paged_forward_kernel<D, FEW, MANY, BF, Q8>, dim3(p.grid()), kPagedThreads, stream, a) != hipSuccess) return FUSED_MHA_ERR_LAUNCH;
   if (!p.shared) return FUSED_MHA_OK;
-  const int rows = a.tokens * a.head, rows_of_group = MANY ? 32 : 1;
-  return launch(paged_join_kernel<D, BF>, dim3((rows + rows_of_group - 1) / rows_of_group), 256, stream, a, p.place_rows(), rows_of_group) == hipSuccess
+  const int rows = a.tokens * a.head;
+  return launch(paged_join_kernel<D, BF>, dim3(p.join_grid(rows)), 256, stream, a, p.place_rows(), p.join_rows(rows)) == hipSuccess
              ? FUSED_MHA_OK : FUSED_MHA_ERR_LAUNCH;
 }
 
@@ -1718,7 +1724,7 @@ int paged_mha_write(const paged_mha_cache* c, const paged_mha_batch* b, const vo
   if (bad_strides(k_st) || bad_strides(v_st)) return FUSED_MHA_ERR_BAD_STRIDE;
   if (misaligned(k) || misaligned(v)) return FUSED_MHA_ERR_MISALIGNED;
   const long tokens = all_tokens(b);
-  if (tokens >= (1L << 30)) return FUSED_MHA_ERR_TOO_LARGE;
+  if ((tokens + 3) / 4 > kMostGroups) return FUSED_MHA_ERR_TOO_LARGE;
   const int bytes = c->cache_type == PAGED_MHA_E4M3 ? 1 : 2;
   WriteArgs a{};
   a.k = (const char*)k, a.v = (const char*)v;
@@ -1746,7 +1752,7 @@ int paged_mha_read(const paged_mha_cache* c, const paged_mha_batch* b, int max_s
   if (max_seqlen <= 0) return FUSED_MHA_ERR_BAD_SHAPE;
   const int rows_of_block = 256 * kReadSteps / (c->d / 8);
   const long rows = (long)max_seqlen * c->kv_head, blocks = (rows + rows_of_block - 1) / rows_of_block;
-  if (rows >= (1L << 30) || blocks * b->batch >= (1L << 30)) return FUSED_MHA_ERR_TOO_LARGE;
+  if (rows >= (1L << 30) || blocks * b->batch > kMostGroups / 2) return FUSED_MHA_ERR_TOO_LARGE;
   const int bytes = c->cache_type == PAGED_MHA_E4M3 ? 1 : 2;
   ReadArgs a{};
   a.kc = (const char*)c->key, a.vc = (const char*)c->value;
@@ -1771,7 +1777,8 @@ static int check_forward(const paged_mha_cache* c, const paged_mha_batch* b, int
   const Launch p = plan(c, b, head, max_new);
   // the line's length fits 62 bits: an item weighs up to four for each key and new token
   const double weight = 4. * ((double)b->table_width * c->page_size + 128 + b->tokens);
-  return p.items >= (1L << 30) || p.items * weight >= 0x1p61 ? FUSED_MHA_ERR_TOO_LARGE : FUSED_MHA_OK;
+  if (p.items >= (1L << 30) || p.items * weight >= 0x1p61) return FUSED_MHA_ERR_TOO_LARGE;
+  return p.grid() > kMostGroups || p.join_grid(all_tokens(b) * head) > kMostGroups ? FUSED_MHA_ERR_TOO_LARGE : FUSED_MHA_OK;
 }
 
 size_t paged_mha_forward_workspace_bytes(const paged_mha_cache* c, const paged_mha_batch* b, int head, int max_new) {

@@ -79,6 +79,20 @@ def test_long_sequences_in_parts(ops, dim, cache, new, group):
     check_attention(ops, batch, True)
 
 
+@pytest.mark.parametrize("cache", paged.CACHES)
+@pytest.mark.parametrize("dim", (64, 128))
+@pytest.mark.parametrize("lengths,new,group,kv_heads", [
+    ([150000], 1, 3, 1), ([70000, 40, 90000], 1, 2, 1), ([33000, 35000], 2, 1, 2), ([3000] * 66, 1, 1, 1), ([200000], 33, 1, 1),
+    ([40000, 45000, 60], 40, 4, 2), ([41000], 200, 2, 1), ([9000] * 18, 35, 1, 1)])
+def test_parts_of_all_work_groups(ops, dim, cache, lengths, new, group, kv_heads):
+    """So many keys that each work group has some: parts up to the last place."""
+    batch = paged.Batch(lengths, new, kv_heads, group, dim, 64, torch.float16, cache, seed=dim)
+    check_attention(ops, batch, True, 0.5)  # few keys have most of the weight
+    if new < 40:
+        batch = paged.Batch(lengths + [5, 64], [new] * len(lengths) + [1, 0], kv_heads, group, dim, 64, torch.bfloat16, cache, packed=True, seed=dim)
+        check_attention(ops, batch, False, 0.5)
+
+
 @pytest.mark.parametrize("count", (65, 130, 4200))
 def test_many_sequences(ops, count):
     """More than a wave looks at together."""
@@ -269,6 +283,25 @@ def test_offsets_past_32_bits(ops, cache):
     k, _ = ops.kv_cache_read(*one.args(), 500, **one.scales())
     if cache == "same":
         assert torch.equal(k[0, 497:500], one.k[0])
+
+
+@pytest.mark.parametrize("new", (1, 70))
+def test_half_a_billion_keys(ops, new):
+    """The same page over and over, then five keys that outweigh all before them: scores of 40, where 2^29 others have 1.1 at most
+    (0.5 * 64 * 0.03 rounded, + 16 times a step), so together 2^29 e^-38.9 / 5 < 2e-9 of the weight.  Probabilities of the five are
+    1 of a sum of 5; the result rounds to 2^-11 of itself."""
+    page, dim, last = 1 << 20, 64, 5
+    g = torch.Generator().manual_seed(6)
+    k = (torch.rand(2 * page, dim, generator=g) * 0.06 - 0.03).half()
+    v = torch.randn(2 * page, dim, generator=g).half()
+    k[page:page + last] = 2.5
+    table = torch.zeros(1, 513, dtype=torch.int32, device="cuda")
+    table[0, 512] = 1
+    lengths = torch.tensor([512 * page + last], dtype=torch.int32, device="cuda")
+    caches = [x.view(2, page, 1, dim).cuda() for x in (k, v)]
+    got = ops.flash_attn_paged_func(torch.full((1, new, 1, dim), 2.0).half().cuda(), *caches, table, lengths).cpu().double()
+    want = v[page:page + last].double().mean(0)
+    assert ((got - want).abs() <= want.abs() * 2.0 ** -11 + 2.0 ** -20 * 4).all()
 
 
 @pytest.mark.parametrize("cache", paged.CACHES)

@@ -136,6 +136,19 @@ def test_refusals_of_write_and_read(lib):
     assert lib.paged_mha_read(c, b, 100, P, P + 2, None) == abi.ERR_MISALIGNED
 
 
+def test_launches_too_large_for_a_grid(lib):
+    """Of 256 threads a work group, 2^32 work items in all at most."""
+    c, b, call = problem(tokens=1 << 27, batch=1)
+    st = ctypes.byref(call["q_st"])
+    assert lib.paged_mha_write(c, b, P, st, P, st, None) == abi.ERR_TOO_LARGE
+    c, b, call = problem(batch=1 << 20)
+    assert lib.paged_mha_read(c, b, 2000, P, P, None) == abi.ERR_TOO_LARGE
+    for heads, width in ((64, 8), (512, 1000)):  # a work group for each item; rows that may have parts
+        c, b, call = problem(batch=1 << 20, tokens=1, kv_head=heads, table_width=width)
+        assert lib.paged_mha_forward_workspace_bytes(c, b, heads, 0) == 0
+        assert lib.paged_mha_forward(c, b, P, st, P, heads, 0, 1.0, 1, 0, P, 1 << 40, None) == abi.ERR_TOO_LARGE
+
+
 def test_python_signatures():
     import flash_attn_v100 as f
     assert str(inspect.signature(f.flash_attn_paged_func)) == (
@@ -323,6 +336,26 @@ int main() {
           if (it.next != it.tiles || it.parts != it.told) return puts("not whole"), 1;
         }
   }
+  puts("ok");
+}
+""")
+    assert out == "ok\n"
+
+
+def test_parts_fit_their_places(tmp_path):
+    """All that begin and end in one of the stretches, none that would go past the last one."""
+    out = host_program(tmp_path, r"""
+int main() {
+  for (int rows : {16, 32, 128})
+    for (int first = 0; first < kPagedGroups; ++first)
+      for (int parts = 1; parts < kPagedGroups + 3; ++parts)
+        for (int row : {0, 1, rows - 1}) {
+          const bool fit = paged_parts_fit(2 * first * rows + row, parts, rows);
+          if (fit != (parts > 1 && first + parts <= kPagedGroups)) return printf("%d %d %d\\n", rows, first, parts), 1;
+          for (int p = 0; fit && p < parts; ++p)
+            if (paged_place(first, p) >= 2 * kPagedGroups) return puts("past"), 1;
+        }
+  if (paged_parts_fit(-1, 2, 16) || paged_parts_fit(0, -5, 16) || paged_parts_fit(0x7fffffff, 0x7fffffff, 128)) return puts("nonsense"), 1;
   puts("ok");
 }
 """)
