@@ -1349,11 +1349,11 @@ __global__ void __launch_bounds__(kPagedThreads, 2) paged_forward_kernel(PagedAr
   constexpr int kManyBytes = MANY ? ManyGeom<D, Q8>::kBytes : 0;
   __shared__ __attribute__((aligned(1024))) char smem[kFewBytes > kManyBytes ? kFewBytes : kManyBytes];
   const PagedArgs& a = args;
-  if (a.zero_rest) {
-    const int rest = min(max(a.ends[a.batch - 1], 0), a.tokens);
-    const long from = (long)rest * a.head * D * 2, to = (long)a.tokens * a.head * D * 2;
-    for (long i = from + ((long)blockIdx.x * blockDim.x + threadIdx.x) * 16; i < to; i += (long)gridDim.x * blockDim.x * 16)
-      *reinterpret_cast<u4v*>(a.o + i) = u4v{0, 0, 0, 0};
+  if (a.zero_rest) {  // in front of the first sequence and behind the last
+    const int first = min(max(a.ends[-1], 0), a.tokens), rest = min(max(a.ends[a.batch - 1], 0), a.tokens);
+    const long row = (long)a.head * D * 2, skip = max(rest - first, 0) * row, to = a.tokens * row - skip;
+    for (long i = ((long)blockIdx.x * blockDim.x + threadIdx.x) * 16; i < to; i += (long)gridDim.x * blockDim.x * 16)
+      *reinterpret_cast<u4v*>(a.o + (i < first * row ? i : i + skip)) = u4v{0, 0, 0, 0};
   }
   touch_args();
   const int lane = threadIdx.x & 63;

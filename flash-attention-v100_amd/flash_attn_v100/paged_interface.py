@@ -10,7 +10,8 @@ contiguous and begin on 16-byte boundaries.
 page_table[b, p // page_size].  ``cache_seqlens`` (batch), int32: how many keys a sequence has, those of its new tokens among
 them; new token i of n is at position cache_seqlens[b] - n + i.  Both stay on the GPU and are read there, so a captured graph
 takes what they hold at its replay.  What is not valid in them never leads out of the tensors: positions behind the table's
-columns, or on a page that the cache does not have, are left out when written, and give NaN when read or attended to.
+columns, or on a page that the cache does not have, are left out when written, and give NaN when read or attended to.  Scales
+other than those that kv_cache_write makes are 2 ** -126 or more, and no NaN.
 
 New tokens come as (batch, seqlen, heads, head_size), all sequences with as many, or packed as (tokens, heads, head_size) with
 ``cu_seqlens`` (batch + 1), int32: sequence b has tokens cu_seqlens[b] .. cu_seqlens[b + 1] - 1.
@@ -35,7 +36,8 @@ def flash_attn_paged_func(q, k_cache, v_cache, page_table, cache_seqlens, softma
     """Attention of new tokens over the cache, which already holds their own keys and values (kv_cache_write).
 
     q has a multiple of the cache's heads: query head h attends to head h // (heads // kv_heads).  causal: a token sees keys up to
-    its own position, otherwise all of its sequence.  Rows that see no key are zero.  softmax_scale: head_size ** -0.5 if None.
+    its own position, otherwise all of its sequence.  Rows that see no key are zero.  Values that a token does not see have a
+    weight of 0: those of later new tokens have to be finite.  softmax_scale: head_size ** -0.5 if None.
     max_seqlen: no sequence has more new tokens (with cu_seqlens; helps to pick the kernel, is not needed for the result).
     out: dense tensor of q's shape to write to; rows of tokens that belong to no sequence stay as they are there, and are zero
     in a tensor made here.  Returns it."""

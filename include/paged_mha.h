@@ -12,9 +12,10 @@
  * What lies in device memory is not known to the host, so the kernels keep to their bounds by themselves:
  *   - a length is taken as 0 below 0; positions past the page table or on a page that is none of the cache's (a number that is
  *     not 0 .. pages-1) are not accessed: paged_mha_write leaves those out, paged_mha_read gives NaN for them, and
- *     paged_mha_forward gives NaN for all rows that would see one;
+ *     paged_mha_forward gives NaN for all rows that would see one, and may for other rows of the same sequence;
  *   - entries of cu_seqlens are taken as within 0 .. tokens; tokens that belong to no sequence are not read, and rows of the
- *     output that belong to none are zeroed or left as they are (paged_mha_forward);
+ *     output that belong to none are zeroed or left as they are (paged_mha_forward).  Where entries decrease, the sequences' rows
+ *     hold any numbers;
  *   - entries of the page table behind a sequence's last key, and what the cache holds there, are not looked at.
  */
 #ifndef PAGED_MHA_H_
@@ -39,7 +40,7 @@ extern "C" {
 /* 8 bits, OCP e4m3 without infinities, with a scale for each position and head: 2^(byte - 127), byte 1 .. 254. */
 #define PAGED_MHA_E4M3 2
 
-/* Element strides; rows of d elements are contiguous and begin on 16-byte boundaries.  slot < 2^24, head < 2^31. */
+/* Element strides; rows of d elements are contiguous and begin on 16-byte boundaries.  slot < 2^24, head < 2^30. */
 typedef struct paged_mha_strides {
   long long page, slot, head;
 } paged_mha_strides;
@@ -84,8 +85,11 @@ int paged_mha_read(const paged_mha_cache *cache, const paged_mha_batch *batch, i
 /*
  * o_i = sum_j softmax_j(scale * q_i . k_j) v_j over the keys j of the sequence; causal != 0: over those up to the token's own
  * position.  head is a multiple of kv_head; query head h has key head h / (head / kv_head).  A row without keys is zero.
+ * Keys that a row does not see do not matter to it, whatever they hold.  Their values have a weight of 0, so that those of later new
+ * tokens have to be finite: 0 times what is not is NaN.
  * o is dense.  max_new: no sequence has more new tokens (0: not known); which kernel is taken goes by it, not the result.
- * zero_rest: rows of o behind those of the last sequence (tokens from cu_seqlens[batch] on) are zeroed instead of left.
+ * zero_rest: rows of o that belong to no sequence (tokens in front of cu_seqlens[0], and from cu_seqlens[batch] on) are zeroed
+ * instead of left.
  * The workspace holds parts of long sequences that several work groups share; its contents do not matter before or after.
  */
 size_t paged_mha_forward_workspace_bytes(const paged_mha_cache *cache, const paged_mha_batch *batch, int head, int max_new);

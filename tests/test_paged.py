@@ -79,6 +79,36 @@ def test_long_sequences_in_parts(ops, dim, cache, new, group):
     check_attention(ops, batch, True)
 
 
+@pytest.mark.parametrize("new", (1, 20))
+def test_tokens_in_front_of_the_first_sequence(ops, new):
+    """Rows that belong to none, as those behind the last one.  max_seqlen: the kernel goes by the tokens in all otherwise, and its
+    roundings with it."""
+    how = {"max_seqlen": max(new, 3)}
+    batch = paged.Batch([70, 300, 90], [new, 2, 3], 1, 4, 64, packed=True)
+    want = ops.flash_attn_paged_func(batch.q, *batch.args(), None, True, cu_seqlens=batch.cu_seqlens, **how)
+    q = torch.cat([torch.full_like(batch.q[:3], float("nan")), batch.q, torch.full_like(batch.q[:2], float("nan"))])
+    spoilt = torch.full_like(q, 7.0)  # most likely what the next call gets
+    del spoilt
+    got = ops.flash_attn_paged_func(q, *batch.args(), None, True, cu_seqlens=batch.cu_seqlens + 3, **how)
+    assert torch.equal(got[3:-2], want) and not got[:3].any() and not got[-2:].any()
+    out = torch.full_like(q, 7.0)
+    ops.flash_attn_paged_func(q, *batch.args(), None, True, cu_seqlens=batch.cu_seqlens + 3, **how, out=out)
+    assert torch.equal(out[3:-2], want) and (out[:3] == 7).all() and (out[-2:] == 7).all()
+
+
+@pytest.mark.parametrize("dim", (64, 128))
+@pytest.mark.parametrize("new", (9, 50))
+@pytest.mark.parametrize("value", (float("nan"), float("inf"), -float("inf")))
+def test_keys_of_later_tokens_do_not_matter(ops, dim, new, value):
+    batch = paged.Batch([new, 333, 64 + new], new, 2, 2, dim, 16, torch.bfloat16)
+    want = ops.flash_attn_paged_func(batch.q, *batch.args(), None, True)
+    for b, m in enumerate(batch.lengths):
+        ids, slots = po.places(batch.page_table.cpu(), 16, b, torch.arange(m - 3, m))
+        batch.k_cache[ids.cuda(), slots.cuda()] = value
+    got = ops.flash_attn_paged_func(batch.q, *batch.args(), None, True)
+    assert torch.equal(got[:, :-3], want[:, :-3])
+
+
 @pytest.mark.parametrize("cache", paged.CACHES)
 @pytest.mark.parametrize("dim", (64, 128))
 @pytest.mark.parametrize("lengths,new,group,kv_heads", [
