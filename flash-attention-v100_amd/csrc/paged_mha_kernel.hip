@@ -1209,12 +1209,12 @@ __device__ __forceinline__ void many_rows(const PagedArgs& a, const Part& w, cha
         if (D == 64) wait_lds_pinned(reads(m + 2));
         else wait_lds(reads(m + 2));
       }
-      if (m < kM) {
-        const int ch = m / (2 * kDB), in = m % (2 * kDB);
-        if (in < kDB) {
+      if constexpr (m < kM) {
+        constexpr int ch = m / (2 * kDB), in = m % (2 * kDB);
+        if constexpr (in < kDB) {
           o[in] = mma32<BF>(frag[m % kLead], __builtin_bit_cast(h8, pf[ch]), o[in]);
         } else {
-          const int n = ch * kDB + in - kDB, rb = n & 1, kk = n >> 1;
+          constexpr int n = ch * kDB + in - kDB, rb = n & 1, kk = n >> 1;
           sn[rb] = mma32<BF>(frag[m % kLead], qf[kk], kk == 0 ? zero : sn[rb]);
         }
         if (m + kLead < kM) frag[m % kLead] = read(m + kLead);
