@@ -468,8 +468,9 @@ __device__ __forceinline__ void few_rows(const PagedArgs& a, const Part& w, char
   constexpr int kLoads = Q8 ? kNC / 2 : kNC;  // of 16 positions: 64 bytes of each
   float2(*const join)[kRows] = reinterpret_cast<float2(*)[kRows]>(smem + kFewWaves * G::kWaveBytes);
 
-  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int m = lane & 15, g = lane >> 4;
+  int lane = threadIdx.x & 63;
+  asm volatile("" : "+v"(lane));  // what depends on it is not kept from item to item, where it goes to scratch
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), m = lane & 15, g = lane >> 4;
   const int rows = w.s.n * a.group, row0 = w.block * kRows, t0 = w.t0;
   const int seen = paged_visible(w.s.keys, w.s.n, (min(rows, row0 + kRows) - 1) / a.group, a.causal);
   const int all_see = paged_visible(w.s.keys, w.s.n, row0 / a.group, a.causal);
@@ -1240,6 +1241,7 @@ __device__ __forceinline__ void many_rows(const PagedArgs& a, const Part& w, cha
   }
   block_barrier();
   if (ntw > 0) scores(0, sA);
+  else asm volatile("" : "=v"(sA[0]), "=v"(sA[1]));  // anything: else the compiler keeps 32 zeros for them, in scratch, from item to item
   int j = 0;
   if (jm > 0) {
     top_wait();
