@@ -172,7 +172,7 @@ struct Blocks {
   // A block of many rows alone on its CU takes 0.55 of the time.  What parts cost (256: a tile): an item more in a stretch, and of
   // many rows to write their sums and to read them again, of up to two in each stretch or of one.
   static constexpr float kAlone = MANY ? 0.58f : 1.f;
-  static constexpr float kStretchesCost = (MANY ? 3 + 14 : 1) * 256, kPartsCost = MANY ? 6 * 256 : 0;
+  static constexpr float kStretchesCost = (MANY ? 3 + 14 : 3) * 256, kPartsCost = MANY ? 6 * 256 : 0;
 };
 // What a work group does of an item.
 struct Part {
@@ -287,9 +287,10 @@ struct Walk {
       // 64 lengths, from the even one up to five times that, by as many lanes: the best for which there are stretches enough
       const float mine_long = even_long * (1.f + lane * (1.f / 16.f)), mine_in = __builtin_amdgcn_rcpf(mine_long);
       const float weight = heaviest(a, mine.n, mine.keys);
-      const int of_mine = B::count(mine.n * a.group) * (int)a.kv_head;
+      const int of_mine = lane < a.batch ? B::count(mine.n * a.group) * (int)a.kv_head : 0;
       int count = 0;
-      for (int b = 0; b < a.batch; ++b)
+#pragma unroll 8
+      for (int b = 0; b < (a.batch + 7) / 8 * 8; ++b)
         count += __builtin_amdgcn_readlane(of_mine, b) * paged_parts(__uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(weight), b)), mine_in);
       const float cost = count <= kCus ? B::kAlone * mine_long + 0.5f * B::kPartsCost : count <= kPagedGroups ? mine_long + B::kPartsCost : INFINITY;
       const float least = -same(max_over_wave(-cost));
