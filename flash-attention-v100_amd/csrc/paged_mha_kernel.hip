@@ -158,7 +158,7 @@ __device__ __forceinline__ long scan_over_wave(long x) {
 // Which blocks a launch has: FEW rows for sequences that have at most kFewRows of them, kManyRows for the others; or all of one
 // kind, with FEW = 0 or MANY = false.
 constexpr int kFewRows = 32, kManyRows = 128;
-template <int FEW, bool MANY>
+template <int FEW, bool MANY, bool Q8>
 struct Blocks {
   static constexpr int kMost = MANY ? kManyRows : FEW;  // rows of a slot
   static __device__ __forceinline__ bool many(int rows) { return MANY && (FEW == 0 || rows > kFewRows); }
@@ -168,7 +168,7 @@ struct Blocks {
   static __device__ __forceinline__ int overhead(int rows) { return many(rows) ? 192 : 64; }
   // Weight of a key: 4 for a block of many rows while another shares its CU.  Beside such blocks those of few rows, which wait for
   // memory, take half of it.
-  static __device__ __forceinline__ int of_key(int rows) { return MANY && FEW && !many(rows) ? 2 : 4; }
+  static __device__ __forceinline__ int of_key(int rows) { return MANY && FEW && Q8 && !many(rows) ? 2 : 4; }
   // A block of many rows alone on its CU takes 0.55 of the time.  What parts cost (256: a tile): an item more in a stretch, and of
   // many rows to write their sums and to read them again, of up to two in each stretch or of one.
   static constexpr float kAlone = MANY ? 0.58f : 1.f;
@@ -1347,7 +1347,7 @@ __device__ __forceinline__ void many_rows(const PagedArgs& a, const Part& w, cha
 // ---------------------------------------------------------------------------
 template <int D, int FEW, bool MANY, bool BF, bool Q8>
 __global__ void __launch_bounds__(kPagedThreads, 2) paged_forward_kernel(PagedArgs args) {
-  using B = Blocks<FEW, MANY>;
+  using B = Blocks<FEW, MANY, Q8>;
   constexpr int kFewBytes = FEW ? kFewWaves * (FewGeom<D, FEW ? FEW / 16 : 1, Q8>::kWaveBytes + FEW * (int)sizeof(float2)) : 0;
   constexpr int kManyBytes = MANY ? ManyGeom<D, Q8>::kBytes : 0;
   __shared__ __attribute__((aligned(1024))) char smem[kFewBytes > kManyBytes ? kFewBytes : kManyBytes];
@@ -1818,7 +1818,7 @@ int paged_mha_forward(const paged_mha_cache* c, const paged_mha_batch* b, const 
   a.c = scale * kLog2e;
   a.causal = causal != 0, a.zero_rest = zero_rest != 0 && a.ends;
   a.shared = p.shared;
-  a.step[0] = paged_step(p.few, head / c->kv_head, p.many ? 2 : 4), a.step[1] = paged_step(kManyRows, head / c->kv_head, 4);
+  a.step[0] = paged_step(p.few, head / c->kv_head, p.many && p.few && bytes == 1 ? 2 : 4), a.step[1] = paged_step(kManyRows, head / c->kv_head, 4);
   if (p.many) fits(c, c->key_strides, bytes, a.k_shift), fits(c, c->value_strides, bytes, a.v_shift);
   return with_types(c, [&](auto d, auto bf, auto q8) {
     constexpr int D = decltype(d)::value;
