@@ -156,7 +156,9 @@ __device__ __forceinline__ long scan_over_wave(long x) {
 }
 
 // Which blocks a launch has: FEW rows for sequences that have at most kFewRows of them, kManyRows for the others; or all of one
-// kind, with FEW = 0 or MANY = false.
+// kind, with FEW = 0 or MANY = false.  A block of many rows multiplies 128 whatever it has, one of few reads its keys for 16 or 32.
+// us of 16 sequences of about 4096 keys, 8 key heads of 128, bf16, in blocks of few rows and of many: 32 rows a key head 57.3, 63.0; 48
+// 79.5, 64.3; 64 81.2, 65.7.  In blocks of 16 and of 32: 4 rows 49.0, 50.5; of 8 sequences 24.2, 25.9; 200 over 200 keys 26.9, 30.5.
 constexpr int kFewRows = 32, kManyRows = 128;
 template <int FEW, bool MANY, bool Q8>
 struct Blocks {
@@ -164,14 +166,20 @@ struct Blocks {
   static __device__ __forceinline__ bool many(int rows) { return MANY && (FEW == 0 || rows > kFewRows); }
   static __device__ __forceinline__ int rows_of_block(int rows) { return many(rows) ? kManyRows : FEW; }
   static __device__ __forceinline__ int count(int rows) { return paged_blocks(rows, rows_of_block(rows)); }
+  // The rest is what is known about time, for sharing it out, timed over 20 batches; figures are us.
   // What an item costs beside its keys, in keys: about three tiles where a block has many rows, one where it has few.
   static __device__ __forceinline__ int overhead(int rows) { return many(rows) ? 192 : 64; }
-  // Weight of a key: 4 for a block of many rows while another shares its CU.  Beside such blocks those of few rows, which wait for
-  // memory, take half of it.
+  // Weight of a key: 4 for a block of many rows while another shares its CU, and for one of few, which waits for memory; out of 8 bits
+  // that takes half as long.  With 2 and 4 for few rows, a chunk of 512 new tokens beside 39 sequences with one, 4000 keys: 16-bit
+  // 105.0, 83.1; 8-bit 69.5, 91.0; two of 500 beside 28 of 8000: 208.2, 170.5; 8-bit 153.8, 159.9.
   static __device__ __forceinline__ int of_key(int rows) { return MANY && FEW && Q8 && !many(rows) ? 2 : 4; }
-  // A block of many rows alone on its CU takes 0.55 of the time.  What parts cost (256: a tile): an item more in a stretch, and of
-  // many rows to write their sums and to read them again, of up to two in each stretch or of one.
+  // A block of many rows alone on its CU takes 0.58 of the time (one of few as long as with another).  With 0.5, 0.58 and 0.7: 512 new
+  // tokens of 8192 88.0, 85.5, 85.6; 900 of 4000 72.9, 71.5, 79.3; three of 300 of 4000 74.0, 73.3, 82.2; 8-bit 91.3, 90.8, 91.4.
   static constexpr float kAlone = MANY ? 0.58f : 1.f;
+  // What parts cost (256: a tile): an item more in a stretch, and of many rows to write their sums and to read them again, of up
+  // to two in each stretch or of one.  Stretches: few rows with 2, 3 and 6 tiles 16 sequences of 4096 50.5, 49.0, 49.0; of 32 rows 62.2,
+  // 57.3, 57.7; many with 8, 17 and 30 900 of 4000 85.8, 71.5, 71.3.  Parts with 2, 6 and 12: 900 of 4000 78.2, 71.5, 71.4; 512 of 8192
+  // 85.4, 85.5, 87.5; four of 200 of 2000 52.2, 43.2, 43.0.
   static constexpr float kStretchesCost = (MANY ? 3 + 14 : 3) * 256, kPartsCost = MANY ? 6 * 256 : 0;
 };
 // What a work group does of an item.
@@ -200,8 +208,11 @@ __device__ __forceinline__ float nearly(long x) { return fmaf((float)(unsigned)(
 __device__ __forceinline__ float nearly(float x, float y) { return x * __builtin_amdgcn_rcpf(y); }
 
 // A work group's items, one after the other (ways to share them: paged_plan.h); all lanes together, each with one of 64 sequences
-// in its registers.  Every work group finds its own from the lengths of all sequences; what it takes for that is time during which
-// no memory is read, so whole numbers of 32 bits serve wherever they can.
+// in its registers.  Every work group finds its own from the lengths of all sequences, in about 2700 cycles and 1900 for an item; that
+// is time during which no memory is read, so whole numbers of 32 bits serve wherever they can.
+// us with stretches, parts, whole items and the way taken: 8 sequences of 4096 keys, 4 rows a key head 24.9, 23.9, 33.9, 24.2; 40 of 3000
+// 78.8, 86.1, 96.1, 79.5; 512 new tokens of 8192 94.2, 85.5, 114.8, 85.5; 2048 of as many 76.5, 57.3, 50.1, 52.0; 731 beside single tokens,
+// 8-bit, 113.3, 141.0, 99.9, 100.9.
 template <typename B>
 struct Walk {
   enum Way { kStretches, kParts, kWhole };
@@ -427,6 +438,10 @@ __device__ __forceinline__ float over_groups_sum(float x) {
 // neighbouring ones to a wave, no barrier between them, a tile of LDS for each wave.  Scores are formed transposed,
 // S^T[keys][rows], so that the 16-bit probabilities are the second product's operand as they are (Geom16).  At the end the waves'
 // sums are joined in LDS.
+//
+// Bound by reading the cache, and for short ones by what waits for what: lengths, pages, keys, the sums of the parts.  4 rows a key
+// head, 8 key heads of 128: 131072 keys of one sequence 103 us, 5.2 TB/s of 6.0 that reads alone reach; 8 of about 4096 24.4 us, 3.8 TB/s,
+// of which 4.5 for the join; 32 of 8192 in 8 bits 78 us, 4.0 TB/s, where the copies by themselves take 76 (128 bytes of each KiB at a time).
 //
 // 16-bit cache: a unit comes to registers while the one before is worked on, then goes to the tile.
 // 8-bit cache: units are copied to LDS as they are, two at a time, and converted where they become operands.  Keys' scales go into
@@ -821,6 +836,10 @@ __device__ __forceinline__ void few_rows(const PagedArgs& a, const Part& w, char
 // forward for equal lengths: softmax(j) with the MFMAs of accumulate(j - 1) and scores(j + 1) between its vector
 // instructions, the running maximum raised only where a tile's probabilities come out too large.  New tokens stand anywhere
 // against the tiles, so up to two tiles of a wave need a mask; they are done after the main loop.
+//
+// Bound by the MFMAs with what stands between them: 4096 new tokens of 32768, 32 heads of 128, fp16 1808 us, 1.14 PFLOP/s of the
+// 1.24 that a large library product reaches; 2048 of 16384 475 us, 1.08 (bf16 446, 1.16; 8-bit cache 530, 0.97; heads of 64 294, 0.88).
+// With few blocks, by the parts' sums, 64 KiB each, and by the beginnings: 512 of 8192 81 us, 0.82 PFLOP/s, 10 of them for the join.
 // ---------------------------------------------------------------------------
 template <int D, bool Q8>
 struct ManyGeom {
@@ -1379,7 +1398,8 @@ __global__ void __launch_bounds__(kPagedThreads, 2) paged_forward_kernel(PagedAr
 // ---------------------------------------------------------------------------
 // Rows whose keys went to several parts.  A slice of D / 4 threads adds up parts of a row, each relative to the largest maximum so
 // far.  A work group has one row, whose parts its slices share, or one for each slice; of those with many parts it then takes
-// one after the other.
+// one after the other.  Bound by being a launch of its own where there is little to join (4 us), by its reads of 64 KiB a part of
+// many rows otherwise (512 parts 10 us, 3.4 TB/s).
 // ---------------------------------------------------------------------------
 constexpr int kJoinAhead = 8;  // parts that a slice asks for at a time
 struct Joined {
@@ -1465,7 +1485,9 @@ __global__ void __launch_bounds__(256) paged_join_kernel(PagedArgs a, int slot_r
 }
 
 // ---------------------------------------------------------------------------
-// Writing: a wave to a token, its lanes over 16 bytes of all key heads' keys, then values.  Bound by its bytes.
+// Writing: a wave to a token, its lanes over 16 bytes of all key heads' keys, then values.  Bound by its bytes: 24576 tokens of 8 key
+// heads of 128 into 8 bits 21.8 us, 4.5 TB/s of 5.0 that a copy reaches (asking for all of a token before its place is known 22.8); 64
+// tokens 3.3 us, less than the call takes on the host.
 // ---------------------------------------------------------------------------
 struct WriteArgs {
   const char *k, *v;
@@ -1548,7 +1570,8 @@ __global__ void __launch_bounds__(256) paged_write_kernel(WriteArgs a) {
 }
 
 // ---------------------------------------------------------------------------
-// Reading: 16 bytes of the result to a lane and step.  Bound by its bytes.
+// Reading: 16 bytes of the result to a lane and step.  Bound by its bytes: 4 x 8192 positions of 8 key heads of 128 out of 8 bits
+// 39 us, 4.9 TB/s of 5.0; 1500 of 12 of 64 3.5 us, less than the call takes.  One row after the other 43.5 and 5.3.
 // ---------------------------------------------------------------------------
 struct ReadArgs {
   const char *kc, *vc;
@@ -1687,7 +1710,8 @@ Launch plan(const paged_mha_cache* c, const paged_mha_batch* b, int head, int ma
   const int least_rows = p.few ? p.few : kManyRows;
   const long blocks = b->cu_seqlens ? b->tokens * group / least_rows + b->batch : b->batch * ((b->tokens * group + least_rows - 1) / least_rows);
   p.items = blocks * c->kv_head;
-  // Items of up to 256 keys are not split: a work group each, unless each would look through a long batch for its own.
+  // Items of up to 256 keys are not split: a work group each, unless each would look through a long batch for its own.  us so and shared:
+  // 64 sequences of up to 64 keys, 8 key heads 6.5, 11.3; of 200 12.2, 15.4; 200 of 200 26.9, 32.3.
   p.shared = (long)b->table_width * c->page_size * 4 > kPagedLeast || (b->cu_seqlens && b->batch > 64);
   return p;
 }

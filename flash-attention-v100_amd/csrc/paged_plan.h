@@ -55,7 +55,8 @@ FMHA_HOST_DEVICE int paged_divide(Int n, Int d) {
 }
 
 // Length of a stretch: the same for up to kPagedGroups of them, which is as many work groups as the device runs at a time, but
-// not so short that a work group has little else to do than to begin and end.
+// not so short that a work group has little else to do than to begin and end.  With 128, 256 and 512 keys at least, us: one token over
+// 1500 keys 10.7, 11.5, 12.0; 64 over 200, 8 key heads, which 128 splits, 16.0, 12.2, 11.6; 200 of those 32.4, 26.9, 26.9.
 constexpr int kPagedGroupsLog = 9, kPagedGroups = 1 << kPagedGroupsLog;
 constexpr int kPagedLeastLog = 10, kPagedLeast = 1 << kPagedLeastLog;  // 256 keys
 FMHA_HOST_DEVICE long paged_stretch(long all) {
