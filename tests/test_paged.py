@@ -154,6 +154,38 @@ def test_strides(ops, dim, cache, layout, new):
     check_attention(ops, batch, True)
 
 
+@pytest.mark.parametrize("cache", paged.CACHES)
+@pytest.mark.parametrize("new", (1, 3))
+@pytest.mark.parametrize("group", (33, 71, 160))
+def test_many_query_heads_to_a_key_head(ops, group, new, cache):
+    """Single tokens in blocks of many rows, and tokens that go over two of them."""
+    batch = paged.Batch([1, 77, 300, 0, 64], new, 1, group, 64, 16, torch.bfloat16, cache, seed=group)
+    check_attention(ops, batch, True)
+    batch = paged.Batch([5, 77, 300], [new, 0, 1], 2, group, 128, 16, torch.float16, cache, packed=True, seed=group)
+    check_attention(ops, batch, True)
+
+
+@pytest.mark.parametrize("hint", (None, 1, 3, 40, 1 << 40))
+@pytest.mark.parametrize("cache", paged.CACHES)
+def test_the_hint_does_not_matter(ops, cache, hint):
+    batch = paged.Batch([70, 40, 500, 9], [1, 40, 17, 3], 2, 4, 128, 16, torch.float16, cache, packed=True)
+    check_attention(ops, batch, True, max_seqlen=hint)
+
+
+@pytest.mark.parametrize("cache", paged.CACHES)
+@pytest.mark.parametrize("new", (1, 40))
+def test_keys_and_values_laid_out_differently(ops, cache, new):
+    """Each cache and scale with strides of its own, rows of the page table apart, q the same for all sequences."""
+    kinds = {name: paged.Batch([100, 65, 333], new, 2, 4, 128, 16, torch.bfloat16, cache, seed=2, layout=name) for name in ("pages", "heads", "beside")}
+    for a, b, c, d in (("pages", "heads", "beside", "heads"), ("beside", "pages", "heads", "pages")):
+        batch = kinds["pages"]
+        batch.k_cache, batch.v_cache, batch.k_scale, batch.v_scale = kinds[a].k_cache, kinds[b].v_cache, kinds[c].k_scale, kinds[d].v_scale
+        width = batch.page_table.shape[1]
+        batch.page_table = torch.cat([batch.page_table, batch.page_table.flip(0) ^ 1], 1)[:, :width]
+        batch.q = batch.q[:1].expand_as(batch.q)
+        check_attention(ops, batch, True)
+
+
 @pytest.mark.parametrize("scale", (0.0, -0.2, 0.9))
 @pytest.mark.parametrize("new", (1, 40))
 def test_scales(ops, scale, new):
