@@ -1800,7 +1800,7 @@ static int check_forward(const paged_mha_cache* c, const paged_mha_batch* b, int
   if (const int rc = check_cache(c, b)) return rc;
   if (head <= 0 || max_new < 0) return FUSED_MHA_ERR_BAD_SHAPE;
   if (head % c->kv_head) return PAGED_MHA_ERR_BAD_GROUP;
-  if (head > (1 << 16) || all_tokens(b) * head >= (1L << 30)) return FUSED_MHA_ERR_TOO_LARGE;
+  if (head > (1 << 16) || all_tokens(b) >= (1L << 30) || all_tokens(b) * head >= (1L << 30)) return FUSED_MHA_ERR_TOO_LARGE;
   const Launch p = plan(c, b, head, max_new);
   // the line's length fits 62 bits: an item weighs up to four for each key and new token
   const double weight = 4. * ((double)b->table_width * c->page_size + 128 + b->tokens);

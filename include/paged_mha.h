@@ -77,7 +77,7 @@ int paged_mha_write(const paged_mha_cache *cache, const paged_mha_batch *batch, 
 
 /*
  * Keys and values as dense (batch, max_seqlen, kv_head, d) tensors of cache->type; zeros behind a sequence's length.
- * cu_seqlens and tokens are not used.
+ * cu_seqlens is not used, tokens only has to be positive.
  */
 int paged_mha_read(const paged_mha_cache *cache, const paged_mha_batch *batch, int max_seqlen, void *key_ptr,
                    void *value_ptr, void *stream);

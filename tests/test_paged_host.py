@@ -149,6 +149,15 @@ def test_launches_too_large_for_a_grid(lib):
         assert lib.paged_mha_forward(c, b, P, st, P, heads, 0, 1.0, 1, 0, P, 1 << 40, None) == abi.ERR_TOO_LARGE
 
 
+def test_sizes_whose_product_wraps(lib):
+    for tokens, batch, heads in ((1 << 30, 1 << 18, 1 << 16), (1 << 30, 1 << 20, 1 << 14), ((1 << 31) - 1, 1 << 20, 1 << 16)):
+        c, b, call = problem(tokens=tokens, batch=batch, kv_head=heads)
+        st = ctypes.byref(call["q_st"])
+        assert lib.paged_mha_forward_workspace_bytes(c, b, heads, 0) == 0
+        assert lib.paged_mha_forward(c, b, P, st, P, heads, 0, 1.0, 1, 0, P, 1 << 40, None) == abi.ERR_TOO_LARGE
+        assert lib.paged_mha_write(c, b, P, st, P, st, None) == abi.ERR_TOO_LARGE
+
+
 def test_python_signatures():
     import flash_attn_v100 as f
     assert str(inspect.signature(f.flash_attn_paged_func)) == (
