@@ -4,7 +4,8 @@ No counterpart in the reference, whose attention is over queries, keys and value
 The cache is two tensors ``k_cache`` and ``v_cache`` of shape (pages, page_size, kv_heads, head_size), page_size a multiple of
 16, head_size 64 or 128, in fp16 or bf16 as q, k and v are, or in torch.float8_e4m3fn with scales ``k_scale`` and ``v_scale`` of
 shape (pages, page_size, kv_heads) in torch.float8_e8m0fnu.  Strides are free as long as rows of head_size elements are
-contiguous and begin on 16-byte boundaries.
+contiguous and begin on 16-byte boundaries; pages that hold head by head (a transpose(1, 2) of such a tensor) are read up to a
+tenth faster.
 
 ``page_table`` (batch, columns), int32: position p of sequence b is slot p % page_size of page
 page_table[b, p // page_size].  ``cache_seqlens`` (batch), int32: how many keys a sequence has, those of its new tokens among
