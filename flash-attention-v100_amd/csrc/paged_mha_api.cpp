@@ -54,7 +54,10 @@ void written(const at::Tensor& x) {
   if (!x.is_inference()) x.unsafeGetTensorImpl()->bump_version();
 }
 
-paged_mha_strides cache_strides(const at::Tensor& x) { return {x.stride(0), x.stride(1), x.stride(2)}; }
+// The stride of a dimension; torch says anything of those of size 1, which lead nowhere.
+int64_t step(const at::Tensor& x, int64_t dim) { return x.size(dim) == 1 ? 0 : x.stride(dim); }
+
+paged_mha_strides cache_strides(const at::Tensor& x) { return {step(x, 0), step(x, 1), step(x, 2)}; }
 
 // Cache and batch as the C interface takes them.
 struct Paged {
@@ -129,10 +132,10 @@ struct TokenOperand {
   at::Tensor x;
   fused_mha_strides st;
   explicit TokenOperand(const at::Tensor& in) : x(in) {
-    auto of = [](const at::Tensor& t) { return fused_mha_strides{t.dim() == 4 ? t.stride(0) : 0, t.stride(-3), t.stride(-2)}; };
+    auto of = [](const at::Tensor& t) { return fused_mha_strides{t.dim() == 4 ? step(t, 0) : 0, step(t, -3), step(t, -2)}; };
     st = of(x);
     if (x.stride(-1) != 1 || ((st.batch | st.seq | st.head) & 7) || (reinterpret_cast<uintptr_t>(x.data_ptr()) & 15u)) {
-      x = x.contiguous();
+      x = x.clone(at::MemoryFormat::Contiguous);  // contiguous() may be the tensor itself, wherever it begins
       st = of(x);
     }
   }

@@ -510,3 +510,56 @@ def test_written_tensors_count_as_changed(ops):
         product.backward()
     with torch.inference_mode():  # tensors without a version
         ops.flash_attn_paged_func(batch.q, *batch.args(), out=torch.empty_like(batch.q), **batch.scales())
+
+
+def off_boundary(x):
+    """The same values, contiguous, one element behind a 16-byte boundary."""
+    room = torch.empty(x.numel() + 1, dtype=x.dtype, device=x.device)
+    y = room[1:].view(x.shape)
+    y.copy_(x)
+    assert y.is_contiguous() and y.data_ptr() % 16 == x.element_size()
+    return y
+
+
+@pytest.mark.parametrize("packed", (False, True))
+@pytest.mark.parametrize("new", (1, 40))
+def test_contiguous_tokens_off_16_byte_boundaries(ops, new, packed):
+    batch = paged.Batch([130, 77, 600], [new] * 3 if packed else new, 2, 2, 64, 16, torch.float16, packed=packed, seed=11)
+    other = paged.Batch([130, 77, 600], [new] * 3 if packed else new, 2, 2, 64, 16, torch.float16, packed=packed, seed=11)
+    ops.kv_cache_write(batch.k, batch.v, *batch.args(), cu_seqlens=batch.cu_seqlens)
+    ops.kv_cache_write(off_boundary(batch.k), off_boundary(batch.v), *other.args(), cu_seqlens=batch.cu_seqlens)
+    for name in ("k_cache", "v_cache"):
+        assert torch.equal(getattr(batch, name).view(torch.int16), getattr(other, name).view(torch.int16))
+    batch.q = off_boundary(batch.q)
+    check_attention(ops, batch, True)
+
+
+def any_stride(x, dim):
+    """The same values, with a stride of a dimension of size 1 that no other one has a multiple of."""
+    strides = list(x.stride())
+    strides[dim] = 1
+    y = x.as_strided(x.shape, strides)
+    assert x.shape[dim] == 1 and torch.equal(x.contiguous().view(torch.uint8), y.contiguous().view(torch.uint8))
+    return y
+
+
+@pytest.mark.parametrize("cache", paged.CACHES)
+@pytest.mark.parametrize("new", (1, 40))
+def test_strides_of_dimensions_of_size_1(ops, new, cache):
+    """They say nothing: one head, one page, one sequence, one token."""
+    batch = paged.Batch([130], new, 1, 1, 64, 160, torch.float16, cache, seed=12)
+    ids = batch.page_table[0, :1].long()
+    for name in ("k_cache", "v_cache", "k_scale", "v_scale"):
+        x = getattr(batch, name)
+        if x is not None:
+            x = x.view(torch.uint8)[ids].view(x.dtype)
+            setattr(batch, name, any_stride(any_stride(x, 2), 0))
+    batch.page_table[0, 0] = 0
+    for dim in (0, 2) + ((1,) if new == 1 else ()):
+        batch.q, batch.k, batch.v = (any_stride(x, dim) for x in (batch.q, batch.k, batch.v))
+    check_attention(ops, batch, True)
+    ops.kv_cache_write(batch.k, batch.v, *batch.args(), **batch.scales())
+    check_attention(ops, batch, True)
+    k, _ = ops.kv_cache_read(*batch.args(), 130, **batch.scales())
+    if cache == "same":
+        assert torch.equal(k[0, -new:], batch.k[0])
