@@ -59,7 +59,7 @@ struct Operand {
     const bool ok = x.stride(3) == 1 && sb >= 0 && sn >= 0 && sh >= 0 && ((sb | sn | sh) & 7) == 0 &&
                     sn < (int64_t(1) << 24) && sh < (int64_t(1) << 31) && (reinterpret_cast<uintptr_t>(ptr) & 15u) == 0;
     if (ok) return;
-    copy = x.contiguous();
+    copy = x.clone(at::MemoryFormat::Contiguous);  // contiguous() may be the tensor itself, wherever it begins
     ptr = copy.data_ptr();
     st = {copy.stride(0), copy.stride(1), copy.stride(2)};
   }

@@ -376,6 +376,31 @@ def test_strided_inputs_python_api():
     assert torch.equal(out2, out.detach())
 
 
+@pytest.mark.parametrize("D", (64, 128))
+def test_contiguous_inputs_off_16_byte_boundaries(D):
+    """Views into a larger buffer, as gradients of parts of a tensor are too; a dimension of size 1 may have any stride."""
+    from flash_attn_v100 import flash_attn_func
+
+    def off_boundary(x):
+        room = torch.empty(x.numel() + 1, dtype=x.dtype, device=x.device)
+        y = room[1:].view(x.shape).copy_(x)
+        assert y.is_contiguous() and y.data_ptr() % 16 == 2
+        return y
+
+    B, H, N = 1, 2, 96
+    q, k, v, do = (x.cuda() for x in ao.make_inputs(B, N, H, D, seed=78))
+    leaves = [x.clone().requires_grad_() for x in (q, k, v)]
+    want = flash_attn_func(*leaves, None, True)
+    want.backward(do)
+    for place in (off_boundary, lambda x: x.as_strided(x.shape, (1, *x.stride()[1:]))):
+        moved = [place(x).requires_grad_() for x in (q, k, v)]
+        got = flash_attn_func(*moved, None, True)
+        got.backward(place(do))
+        assert torch.equal(got, want)
+        for a, b in zip(moved, leaves):
+            assert torch.equal(a.grad, b.grad)
+
+
 def test_hip_graph_capture_and_replay():
     """The extension only launches kernels on the current stream (no synchronisation, no memset),
     so forward + backward can be captured into a graph; every replay must equal the eager result."""
