@@ -41,11 +41,14 @@ void check_devices(const at::Tensor& k_cache, std::initializer_list<const at::Te
 }
 
 // There is no gradient through a cache: better an error than a result without one.
-void check_no_grad(std::initializer_list<const at::Tensor*> xs) {
-  for (const at::Tensor* x : xs) {
-    TORCH_CHECK(!(at::GradMode::is_enabled() && x->requires_grad()) && !x->_fw_grad(/*level=*/0).defined(),
+void check_no_grad(std::initializer_list<const at::Tensor*> xs, std::initializer_list<const OptTensor*> ys) {
+  auto check = [](const at::Tensor& x) {
+    TORCH_CHECK(!(at::GradMode::is_enabled() && x.requires_grad()) && !x._fw_grad(/*level=*/0).defined(),
                 "the paged cache has no gradients: call it under torch.no_grad() or with detached tensors");
-  }
+  };
+  for (const at::Tensor* x : xs) check(*x);
+  for (const OptTensor* y : ys)
+    if (y->has_value()) check(**y);
   TORCH_CHECK(!torch::jit::tracer::isTracing(), "the paged cache is not supported under torch.jit.trace");
 }
 
@@ -147,7 +150,7 @@ at::Tensor paged_attention(const at::Tensor& q, const at::Tensor& k_cache, const
                            const at::Tensor& cache_seqlens, c10::optional<double> softmax_scale, bool is_causal,
                            const OptTensor& cu_seqlens, c10::optional<int64_t> max_seqlen, const OptTensor& k_scale,
                            const OptTensor& v_scale, const OptTensor& out_) {
-  check_no_grad({&q, &k_cache, &v_cache});
+  check_no_grad({&q, &k_cache, &v_cache}, {&k_scale, &v_scale, &out_});
   Paged p(k_cache, v_cache, page_table, cache_seqlens, cu_seqlens, k_scale, v_scale, q.scalar_type());
   p.set_tokens(q, "query", 0);
   const int64_t heads = q.size(-2);
@@ -179,7 +182,7 @@ at::Tensor paged_attention(const at::Tensor& q, const at::Tensor& k_cache, const
 void cache_write(const at::Tensor& k, const at::Tensor& v, const at::Tensor& k_cache, const at::Tensor& v_cache,
                  const at::Tensor& page_table, const at::Tensor& cache_seqlens, const OptTensor& cu_seqlens, const OptTensor& k_scale,
                  const OptTensor& v_scale) {
-  check_no_grad({&k, &v, &k_cache, &v_cache});
+  check_no_grad({&k, &v, &k_cache, &v_cache}, {&k_scale, &v_scale});
   Paged p(k_cache, v_cache, page_table, cache_seqlens, cu_seqlens, k_scale, v_scale, k.scalar_type());
   p.set_tokens(k, "key", p.cache.kv_head);
   p.set_tokens(v, "value", p.cache.kv_head);
@@ -208,7 +211,7 @@ void cache_write(const at::Tensor& k, const at::Tensor& v, const at::Tensor& k_c
 std::tuple<at::Tensor, at::Tensor> cache_read(const at::Tensor& k_cache, const at::Tensor& v_cache, const at::Tensor& page_table,
                                               const at::Tensor& cache_seqlens, int64_t max_seqlen, const OptTensor& k_scale,
                                               const OptTensor& v_scale, c10::optional<at::ScalarType> dtype) {
-  check_no_grad({&k_cache, &v_cache});
+  check_no_grad({&k_cache, &v_cache}, {&k_scale, &v_scale});
   const bool q8 = k_cache.scalar_type() == at::kFloat8_e4m3fn;
   Paged p(k_cache, v_cache, page_table, cache_seqlens, c10::nullopt, k_scale, v_scale,
           dtype.has_value() ? *dtype : q8 ? at::kHalf : k_cache.scalar_type());

@@ -17,7 +17,7 @@ other than those that kv_cache_write makes are 2 ** -126 or more, and no NaN.
 New tokens come as (batch, seqlen, heads, head_size), all sequences with as many, or packed as (tokens, heads, head_size) with
 ``cu_seqlens`` (batch + 1), int32: sequence b has tokens cu_seqlens[b] .. cu_seqlens[b + 1] - 1.
 
-The three calls have no gradients and refuse inputs that ask for them.
+The three calls have no gradients and refuse tensors that ask for them, those that they write to among them.
 """
 import torch  # noqa: F401  (before the kernels, so that they bind to the HIP runtime it has loaded)
 

@@ -247,6 +247,27 @@ def test_refusals_of_cache_calls_in_python():
         f.kv_cache_read(*b.args(), 10, dtype=torch.bfloat16)
 
 
+def test_written_and_read_tensors_that_ask_for_gradients_are_refused():
+    """The output among them: it would go on with the graph of what it held before.  Without gradients the next check is reached."""
+    import flash_attn_v100 as f
+    b = paged.Batch([40, 50, 60], 2, 2, 2, 64, 16, torch.float16, "e4m3", device="cpu")
+    leaf = torch.empty_like(b.q, requires_grad=True)
+    scale = b.k_scale.clone().requires_grad_()
+    for change in ({"out": leaf}, {"out": leaf * 1}, {"k_scale": scale}, {"v_scale": scale}):
+        with pytest.raises(RuntimeError, match="no gradients"):
+            call(b, **change)
+        with torch.no_grad(), pytest.raises(RuntimeError, match="must be on the GPU"):
+            call(b, **change)
+    with pytest.raises(RuntimeError, match="no gradients"):
+        f.kv_cache_write(b.k, b.v, *b.args(), k_scale=scale, v_scale=b.v_scale)
+    with pytest.raises(RuntimeError, match="no gradients"):
+        f.kv_cache_read(*b.args(), 10, k_scale=b.k_scale, v_scale=scale)
+    with torch.autograd.forward_ad.dual_level():
+        dual = torch.autograd.forward_ad.make_dual(torch.empty_like(b.q), torch.ones_like(b.q))
+        with pytest.raises(RuntimeError, match="no gradients"):
+            call(b, out=dual)
+
+
 def test_oracle_rounds_as_torch_does():
     """The oracle's 8-bit values against torch's conversion of x / 2^e, which is exact, and its scales against their definition."""
     g = torch.Generator().manual_seed(0)
