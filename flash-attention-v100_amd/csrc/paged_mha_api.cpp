@@ -52,6 +52,13 @@ void check_no_grad(std::initializer_list<const at::Tensor*> xs, std::initializer
   TORCH_CHECK(!torch::jit::tracer::isTracing(), "the paged cache is not supported under torch.jit.trace");
 }
 
+// A tensor that is written shares no memory with those that are read: work groups read lengths and pages at any time.
+void check_apart(const at::Tensor& out, std::initializer_list<const at::Tensor*> xs, std::initializer_list<const OptTensor*> ys) {
+  for (const at::Tensor* x : xs) at::assert_no_overlap(out, *x);
+  for (const OptTensor* y : ys)
+    if (y->has_value()) at::assert_no_overlap(out, **y);
+}
+
 // For autograd, which holds tensors that were saved before.
 void written(const at::Tensor& x) {
   if (!x.is_inference()) x.unsafeGetTensorImpl()->bump_version();
@@ -161,7 +168,7 @@ at::Tensor paged_attention(const at::Tensor& q, const at::Tensor& k_cache, const
     TORCH_CHECK(out_->scalar_type() == q.scalar_type(), "Output must have the same dtype as inputs");
     TORCH_CHECK(out_->is_contiguous(), "Output tensor must be contiguous");
     TORCH_CHECK(out_->sizes() == q.sizes(), "out must have the shape of q");
-    for (const at::Tensor* x : {&q, &k_cache, &v_cache}) at::assert_no_overlap(*out_, *x);
+    check_apart(*out_, {&q, &k_cache, &v_cache, &page_table, &cache_seqlens}, {&cu_seqlens, &k_scale, &v_scale});
   }
   check_devices(k_cache, {&q, &v_cache, &page_table, &cache_seqlens}, {&cu_seqlens, &k_scale, &v_scale, &out_});
   const api::OnDeviceOf device_guard(q);
@@ -187,16 +194,13 @@ void cache_write(const at::Tensor& k, const at::Tensor& v, const at::Tensor& k_c
   p.set_tokens(k, "key", p.cache.kv_head);
   p.set_tokens(v, "value", p.cache.kv_head);
   TORCH_CHECK(k.sizes() == v.sizes(), "key and value must have the same shape");
-  at::assert_no_overlap(k_cache, v_cache);
-  for (const at::Tensor* x : {&k_cache, &v_cache}) {
-    at::assert_no_internal_overlap(*x);
-    at::assert_no_overlap(*x, k);
-    at::assert_no_overlap(*x, v);
-  }
+  for (const at::Tensor* x : {&k_cache, &v_cache}) at::assert_no_internal_overlap(*x);
+  check_apart(k_cache, {&v_cache, &k, &v, &page_table, &cache_seqlens}, {&cu_seqlens, &k_scale, &v_scale});
+  check_apart(v_cache, {&k, &v, &page_table, &cache_seqlens}, {&cu_seqlens, &k_scale, &v_scale});
   if (k_scale.has_value()) {
-    at::assert_no_internal_overlap(*k_scale);
-    at::assert_no_internal_overlap(*v_scale);
-    at::assert_no_overlap(*k_scale, *v_scale);
+    for (const OptTensor* x : {&k_scale, &v_scale}) at::assert_no_internal_overlap(**x);
+    check_apart(*k_scale, {&*v_scale, &k, &v, &page_table, &cache_seqlens}, {&cu_seqlens});
+    check_apart(*v_scale, {&k, &v, &page_table, &cache_seqlens}, {&cu_seqlens});
   }
   check_devices(k_cache, {&k, &v, &v_cache, &page_table, &cache_seqlens}, {&cu_seqlens, &k_scale, &v_scale});
   const api::OnDeviceOf device_guard(k_cache);

@@ -268,6 +268,34 @@ def test_written_and_read_tensors_that_ask_for_gradients_are_refused():
             call(b, out=dual)
 
 
+def sharing(x, y):
+    """Tensors like both, that share their first bytes."""
+    room = torch.zeros(max(x.numel() * x.element_size(), y.numel() * y.element_size()) + 16, dtype=torch.uint8)
+    return [room[:t.numel() * t.element_size()].view(t.dtype).view(t.shape) for t in (x, y)]
+
+
+@pytest.mark.parametrize("packed", (False, True))
+def test_written_tensors_that_share_memory_with_others_are_refused(packed):
+    """Each pair of a tensor that is written and one that is read, or is written too."""
+    import flash_attn_v100 as f
+    b = paged.Batch([40, 50, 60], [2] * 3 if packed else 2, 2, 2, 64, 16, torch.float16, "e4m3", device="cpu", packed=packed)
+    tensors = {"out": torch.empty_like(b.q), "q": b.q, "k": b.k, "v": b.v, "k_cache": b.k_cache, "v_cache": b.v_cache,
+               "page_table": b.page_table, "cache_seqlens": b.cache_seqlens, **b.scales()}
+    if packed:
+        tensors["cu_seqlens"] = b.cu_seqlens
+    attention = set(inspect.signature(f.flash_attn_paged_func).parameters) & set(tensors)
+    write = set(inspect.signature(f.kv_cache_write).parameters) & set(tensors)
+    for function, names, outputs in ((f.flash_attn_paged_func, attention, ["out"]),
+                                     (f.kv_cache_write, write, ["k_cache", "v_cache", "k_scale", "v_scale"])):
+        for output in outputs:
+            for other in names - {output}:
+                shared = dict(zip((output, other), sharing(tensors[output], tensors[other])))
+                with pytest.raises(RuntimeError, match="memory"):
+                    function(**{name: shared.get(name, tensors[name]) for name in names})
+        with pytest.raises(RuntimeError, match="must be on the GPU"):
+            function(**{name: tensors[name] for name in names})
+
+
 def test_oracle_rounds_as_torch_does():
     """The oracle's 8-bit values against torch's conversion of x / 2^e, which is exact, and its scales against their definition."""
     g = torch.Generator().manual_seed(0)
