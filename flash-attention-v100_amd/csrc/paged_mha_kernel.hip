@@ -446,7 +446,8 @@ __device__ __forceinline__ float over_groups_sum(float x) {
 // 16-bit cache: a unit comes to registers while the one before is worked on, then goes to the tile.
 // 8-bit cache: units are copied to LDS as they are, two at a time, and converted where they become operands.  Keys' scales go into
 // the conversion.  Values' scales, which differ along the second product's sum, go into the probabilities: exp2(t + e - m') with
-// the value's exponent e and a maximum m' of its own of t + e, so that what counts most is 1 whatever the scales are.
+// the value's exponent e and a maximum m' of its own of t + e, so that what counts most is 1 whatever the scales are; in fp16 2^14,
+// which leaves values of up to 2^-28 of the largest scale their probabilities' 11 bits, and drops none before 2^-39.
 // ---------------------------------------------------------------------------
 constexpr int kPagedThreads = 256;
 constexpr int kFewWaves = kPagedThreads / 64;
@@ -661,6 +662,7 @@ __device__ __forceinline__ void few_rows(const PagedArgs& a, const Part& w, char
     // Chunk c of 16 bytes of row r16 of rows 16 R .. lies at (c ^ swz(r16 >> 2) ^ 2 R) * 16 of the row's 64 bytes, so that neither
     // reads below meet in a bank.
     const int col = (q4 ^ swz(r16 >> 2)) * 16;
+    constexpr float kUp = BF ? 0.f : 14.f;  // the largest probability's exponent
     constexpr int kBack = 960 * (kLoads - 1), kOps = 4 * kLoads + 1;  // see copy16_blocks; copies of a unit
     auto copy = [&](const char* from, int off, unsigned to) __attribute__((always_inline)) {
       if constexpr (kLoads == 1) copy16(wave_uniform(from), off, smem + __builtin_amdgcn_readfirstlane(to - lds0) + wave * G::kWaveBytes);
@@ -753,6 +755,7 @@ __device__ __forceinline__ void few_rows(const PagedArgs& a, const Part& w, char
 #pragma unroll
         for (int e = 0; e < 8; ++e) t[e] += e8[e];
         alpha[cb] = raise(t, mv[cb], from);
+        from -= kUp;
         moved |= alpha[cb] != 1.f;
 #pragma unroll
         for (int e = 0; e < 4; ++e) pf[cb][e] = pack2<BF>(fast_exp2(t[2 * e] - from), fast_exp2(t[2 * e + 1] - from));
@@ -772,10 +775,10 @@ __device__ __forceinline__ void few_rows(const PagedArgs& a, const Part& w, char
       staged_rows_read();  // the slot has been read
       if (u + 2 < u1) ask(u + 2, lds0 + slot);
     }
-    // to the scale of the sums: the exponents are at most the largest of the scales apart
+    // back to the scale of the sums: the exponents are at most the largest of the scales apart
 #pragma unroll
     for (int cb = 0; cb < CB; ++cb) {
-      const float f = mc[cb] == -INFINITY ? 0.f : fast_exp2(mv[cb] - mc[cb]);
+      const float f = mc[cb] == -INFINITY ? 0.f : fast_exp2(mv[cb] - mc[cb] - kUp);
 #pragma unroll
       for (int db = 0; db < kDB; ++db) o[cb][db] *= f;
     }

@@ -563,3 +563,41 @@ def test_strides_of_dimensions_of_size_1(ops, new, cache):
     k, _ = ops.kv_cache_read(*batch.args(), 130, **batch.scales())
     if cache == "same":
         assert torch.equal(k[0, -new:], batch.k[0])
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("dim", (64, 128))
+@pytest.mark.parametrize("less", (12, 20, 26))
+@pytest.mark.parametrize("new,group", [(1, 4), (5, 5), (20, 4)])
+def test_values_of_very_different_scales(ops, new, group, less, dim, dtype):
+    """Out of 8 bits, rows of values up to 57344 in one half of the features beside rows 2^-less as large in the other half, which
+    are not to be lost.  Beside what every call is off by, blocks of few rows round p_j 2^e_j to fp16 with steps of 2^-24, where the largest
+    is 2^14, before it is multiplied with the value's 8 bits y_j: half a step is 2^-39 of the largest.  Blocks of many rows round p_j the
+    same where the largest is 1 or more: 2^-25, times the value."""
+    batch = paged.Batch([300, 40, 3000], new, 2, group, dim, 16, dtype, "e4m3", seed=less)
+    g = torch.Generator().manual_seed(less)
+    shape = batch.v_cache.shape
+    rows = (torch.rand(shape, generator=g) * 0.75 + 0.25) * 57344
+    small = (torch.rand(shape[:3], generator=g) < 0.5)[..., None]
+    first = torch.arange(dim) < dim // 2
+    rows = torch.where(small, rows * 2.0 ** -less, rows).masked_fill(small == first, 0.0).to(dtype)
+    y, e = po.to_e4m3(rows)
+    batch.v_cache.copy_(y.float().to(torch.float8_e4m3fn))
+    batch.v_scale.view(torch.uint8).copy_((e + 127).to(torch.uint8))
+    results = po.paged_attention(batch.q, *batch.args(), None, True, **batch.scales())
+    want = results[0]
+    tolerance = po.attention_tolerance(dtype, dim, *results, 3000, 0.0)
+    if dtype == torch.float16:
+        for b, m in enumerate(batch.lengths):
+            k = po.held(batch.k_cache, batch.k_scale, batch.page_table, b, m)
+            ids, slots = po.places(batch.page_table, 16, b, torch.arange(m))
+            for h in range(batch.heads):
+                s = batch.q[b, :, h].cpu().double() @ k[:, h // group].t() * dim ** -0.5
+                p = torch.softmax(s.masked_fill(torch.arange(m) > m - new + torch.arange(new)[:, None], -torch.inf), -1)
+                ys, es = y[ids, slots, h // group], e[ids, slots, h // group]
+                if new * group <= 32:
+                    tolerance[b, :, h] += 2.0 ** -39 * (p * torch.pow(2.0, es.double())).amax(-1, keepdim=True) * ys.abs().sum(0)
+                else:
+                    tolerance[b, :, h] += 2.0 ** -25 * p.amax(-1, keepdim=True) * (ys * torch.pow(2.0, es.double())[:, None]).abs().sum(0)
+    got = ops.flash_attn_paged_func(batch.q, *batch.args(), None, True, **batch.scales()).cpu().double()
+    assert ((got - want).abs() <= tolerance).all(), float(((got - want).abs() / tolerance).max())
