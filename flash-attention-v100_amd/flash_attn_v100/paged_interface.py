@@ -37,8 +37,8 @@ def flash_attn_paged_func(q, k_cache, v_cache, page_table, cache_seqlens, softma
     """Attention of new tokens over the cache, which already holds their own keys and values (kv_cache_write).
 
     q has a multiple of the cache's heads: query head h attends to head h // (heads // kv_heads).  causal: a token sees keys up to
-    its own position, otherwise all of its sequence.  Rows that see no key are zero.  Values that a token does not see have a
-    weight of 0: those of later new tokens have to be finite.  softmax_scale: head_size ** -0.5 if None.
+    its own position, otherwise all of its sequence.  Rows that see no key are zero.  Keys that a token does not see do not matter to
+    it, whatever they and their values hold.  softmax_scale: head_size ** -0.5 if None.
     max_seqlen: no sequence has more new tokens (with cu_seqlens; helps to pick the kernel, is not needed for the result).
     out: dense tensor of q's shape to write to; rows of tokens that belong to no sequence stay as they are there, and are zero
     in a tensor made here.  Returns it."""

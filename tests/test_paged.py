@@ -601,3 +601,46 @@ def test_values_of_very_different_scales(ops, new, group, less, dim, dtype):
                     tolerance[b, :, h] += 2.0 ** -25 * p.amax(-1, keepdim=True) * (ys * torch.pow(2.0, es.double())[:, None]).abs().sum(0)
     got = ops.flash_attn_paged_func(batch.q, *batch.args(), None, True, **batch.scales()).cpu().double()
     assert ((got - want).abs() <= tolerance).all(), float(((got - want).abs() / tolerance).max())
+
+
+@pytest.mark.parametrize("cache", paged.CACHES)
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("dim", (64, 128))
+@pytest.mark.parametrize("new,group", [(1, 4), (3, 2), (7, 4), (9, 9), (50, 1), (200, 2)])
+def test_values_of_later_tokens_do_not_matter(ops, new, group, dim, dtype, cache):
+    """Infinite and NaN values of the last three keys: rows that see them have them, with all other features bit by bit as without; the
+    others do not change at all."""
+    batch = paged.Batch([5, 31, 32, 33, 64, 65, 130, 333, 4100], new, 2, group, dim, 16, dtype, cache, seed=new)
+    for causal in (True, False):
+        want = ops.flash_attn_paged_func(batch.q, *batch.args(), None, causal, **batch.scales())
+        assert torch.isfinite(want).all()
+        clean = batch.v_cache.clone()
+        for back, first, end, value in ((3, 0, 16, "inf"), (2, 8, 24, "-inf"), (1, 20, 32, "nan")):
+            for b, m in enumerate(batch.lengths):
+                ids, slots = po.places(batch.page_table, 16, b, torch.tensor([m - back]))
+                row = batch.v_cache[int(ids), int(slots)]
+                if cache == "same":
+                    row[:, first:end] = float(value)
+                else:  # no infinities
+                    row.view(torch.uint8)[:, first:end] = 0x7f if back > 1 else 0xff
+                sees = torch.arange(new, device="cuda") + m - new >= m - back if causal else torch.ones(new, dtype=torch.bool, device="cuda")
+                want[b, sees, :, first:end] += float(value if cache == "same" else "nan")
+        got = ops.flash_attn_paged_func(batch.q, *batch.args(), None, causal, **batch.scales())
+        assert torch.equal(got.isnan(), want.isnan())
+        assert torch.equal(got.masked_fill(got.isnan(), 0), want.masked_fill(want.isnan(), 0))
+        batch.v_cache.copy_(clean)
+
+
+@pytest.mark.parametrize("dim", (64, 128))
+@pytest.mark.parametrize("new,group", [(1, 4), (40, 2)])
+def test_values_of_later_tokens_in_packed_batches(ops, new, group, dim):
+    """Single tokens and chunks, split over work groups: tokens before the spoilt one as without it."""
+    batch = paged.Batch([9000, 700, 300], [new, 1, 65], 2, group, dim, 32, torch.bfloat16, packed=True, seed=dim)
+    want = ops.flash_attn_paged_func(batch.q, *batch.args(), None, True, cu_seqlens=batch.cu_seqlens)
+    ends = batch.cu_seqlens.tolist()[1:]
+    for b, m in enumerate(batch.lengths):
+        ids, slots = po.places(batch.page_table, 32, b, torch.tensor([m - 1]))
+        batch.v_cache[int(ids), int(slots)] = float("inf")
+        want[ends[b] - 1] = float("inf")
+    got = ops.flash_attn_paged_func(batch.q, *batch.args(), None, True, cu_seqlens=batch.cu_seqlens)
+    assert torch.equal(got, want)
