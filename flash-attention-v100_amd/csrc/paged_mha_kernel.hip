@@ -193,6 +193,12 @@ struct Part {
   Sequence s;
 };
 
+// What stands for a token's row that has no score above -inf: 0 if it sees no key, `other` if all that it sees have a score of -inf,
+// over which a softmax is NaN.
+__device__ __forceinline__ float of_no_score(const Part& w, int token, bool causal, float other) {
+  return paged_visible(w.s.keys, w.s.n, token, causal) > 0 ? other : 0.f;
+}
+
 __device__ __forceinline__ float max_over_wave(float x) {
   auto turned = [](float y, auto by) __attribute__((always_inline)) {  // inside rows of 16 lanes
     return __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(y), 0x120 + decltype(by)::value, 15, 15, true));
@@ -920,12 +926,12 @@ __device__ __forceinline__ void few_rows(const PagedArgs& a, const Part& w, char
     }
     if (w.whole) {
       const int token = (row0 + row) / a.group, head = w.head * (int)a.group + (row0 + row - token * a.group);
-      const float inv = sum == 0.f ? 0.f : 1.f / sum;
+      const float inv = sum == 0.f ? of_no_score(w, token, a.causal, NAN) : 1.f / sum;
       store4<BF>(a.o + (((long)(w.s.first + token) * a.head + head) * D + piece * 4) * 2, x * inv);
     } else {
       const long at = (long)w.place * slot_rows + row;
       *reinterpret_cast<f4v*>(a.part_o + at * D + piece * 4) = x;
-      if (piece == 0) a.part_ml[at] = float2{mx, sum};
+      if (piece == 0) a.part_ml[at] = float2{mx, sum == 0.f ? of_no_score(w, (row0 + row) / a.group, a.causal, 1.f) : sum};
     }
   }
 }
@@ -1465,14 +1471,16 @@ __device__ __forceinline__ void many_rows(const PagedArgs& a, const Part& w, cha
   const int lane = lane_now();
   float l_tot = l_run + other_half(l_run);
   if (bad_pages[0] | bad_pages[1] | bad_pages[2] | bad_pages[3]) l_tot = NAN;
-  const float f = !w.whole ? 1.f : l_tot == 0.f ? 0.f : 1.f / l_tot;
+  const int my_token = min(row0w + (lane & 31), rows - 1) / z.group;
+  const float none = l_tot == 0.f ? of_no_score(w, my_token, z.causal, w.whole ? NAN : 1.f) : 0.f;
+  const float f = !w.whole ? 1.f : l_tot == 0.f ? none : 1.f / l_tot;
   char* const stage = smem + wave * (kResident * M::kPitch);
   const long slot0 = (long)w.place * kManyRows + wave * kResident;
   if (z.shared && w.opens && lane < kResident && row0w + lane < rows) {
     const int row = row0w + lane, token = row / z.group, head = w.head * (int)z.group + row - token * (int)z.group;
     z.places[(w.s.first + token) * z.head + head] = int2{2 * w.stretch * kManyRows + wave * kResident + lane, w.parts};
   }
-  if (!w.whole && lane < kResident && row0w + lane < rows) z.part_ml[slot0 + lane] = float2{mc, l_tot};
+  if (!w.whole && lane < kResident && row0w + lane < rows) z.part_ml[slot0 + lane] = l_tot == 0.f ? float2{-INFINITY, none} : float2{mc, l_tot};
 #pragma unroll
   for (int half = 0; half < D / 64; ++half) {
 #pragma unroll
@@ -1549,9 +1557,10 @@ struct Joined {
   float m, l;
   f4v x;
 };
+// A part whose maximum is -inf has sums of 0, and 1 in the place of l if the row sees keys.
 __device__ __forceinline__ void join_in(Joined& r, float m, float l, f4v x, float mx) {
   const float f = m == -INFINITY ? 0.f : fast_exp2(m - mx);
-  r.l += l * f;  // NaN from a bad page stays
+  r.l += l * (mx == -INFINITY ? 1.f : f);  // NaN from a bad page stays
   r.x += x * f;
 }
 template <int D>
@@ -1596,7 +1605,7 @@ __global__ void __launch_bounds__(256) paged_join_kernel(PagedArgs a, int slot_r
     return r;
   };
   auto store = [&](int row, const Joined& r) __attribute__((always_inline)) {
-    store4<BF>(a.o + ((long)row * D + piece * 4) * 2, r.x * (r.l == 0.f ? 0.f : 1.f / r.l));
+    store4<BF>(a.o + ((long)row * D + piece * 4) * 2, r.x * (r.l == 0.f ? 0.f : r.m == -INFINITY ? NAN : 1.f / r.l));
   };
   const int row0 = blockIdx.x * rows_of_group;
   if (rows_of_group > 1) {

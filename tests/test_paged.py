@@ -644,3 +644,35 @@ def test_values_of_later_tokens_in_packed_batches(ops, new, group, dim):
         want[ends[b] - 1] = float("inf")
     got = ops.flash_attn_paged_func(batch.q, *batch.args(), None, True, cu_seqlens=batch.cu_seqlens)
     assert torch.equal(got, want)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("dim", (64, 128))
+@pytest.mark.parametrize("new,group,packed", [(1, 4, False), (6, 4, False), (40, 2, False), (20, 3, True)])
+def test_scores_of_minus_infinity(ops, new, group, packed, dim, dtype):
+    """Keys with such scores have no weight beside others; a softmax over none but those is NaN, also where parts of it are joined, while a
+    row that sees no key is zero."""
+    lengths = [40, 300, 9000, 40, 300, 9000, 9000, max(new // 2, 1), 0]
+    batch = paged.Batch(lengths, [new] * len(lengths) if packed else new, 2, group, dim, 16, dtype, packed=packed, seed=new)
+    batch.q.abs_()
+    none = (0, 1, 2)  # sequences without any other scores
+    for b, m in enumerate(lengths):
+        at = torch.arange(m) if b in none else torch.arange(0, m, 2) if b < 6 else torch.arange(m // 2) if b == 6 else torch.arange(0)
+        ids, slots = po.places(batch.page_table, 16, b, at)
+        batch.k_cache[ids.cuda(), slots.cuda(), :, 3] = -float("inf")
+    got = ops.flash_attn_paged_func(batch.q, *batch.args(), None, False, cu_seqlens=batch.cu_seqlens).cpu().double()
+    got = got.view(len(lengths), new, batch.heads, dim)
+    causal = ops.flash_attn_paged_func(batch.q, *batch.args(), None, True, cu_seqlens=batch.cu_seqlens).cpu().double()
+    causal = causal.view(len(lengths), new, batch.heads, dim)
+    for b, m in enumerate(lengths):
+        q = batch.q.view(len(lengths), new, batch.heads, dim)[b]
+        k, v = (po.held(c, None, batch.page_table, b, m) for c in (batch.k_cache, batch.v_cache))
+        if b in none:
+            assert got[b].isnan().all()
+            first = max(new - m, 0)
+            assert causal[b, first:].isnan().all() and not causal[b, :first].any()
+            continue
+        want, weight, _ = po.attention(q, k, v, dim ** -0.5, False)
+        size = po.attention(q, k.masked_fill(k.isinf(), 0), v, dim ** -0.5, False)[2]
+        v_max = float(v.abs().max()) if m else 0.0
+        assert ((got[b] - want).abs() <= po.attention_tolerance(dtype, dim, want, weight, size, max(m, 1), v_max)).all()
