@@ -889,7 +889,7 @@ __device__ __forceinline__ void few_rows(const PagedArgs& a, const Part& w, char
 
   if (a.shared && w.opens && threadIdx.x < kRows && row0 + (int)threadIdx.x < rows) {
     const int row = row0 + threadIdx.x, token = row / a.group, head = w.head * (int)a.group + row - token * (int)a.group;
-    a.places[(w.s.first + token) * a.head + head] = int2{2 * w.stretch * slot_rows + (int)threadIdx.x, w.parts};
+    a.places[(w.s.first + token) * a.head + head] = int2{paged_first_row(w.stretch, w.parts, slot_rows) + (int)threadIdx.x, w.parts};
   }
   // the waves' sums, relative to the largest maximum
 #pragma unroll
@@ -1478,7 +1478,7 @@ __device__ __forceinline__ void many_rows(const PagedArgs& a, const Part& w, cha
   const long slot0 = (long)w.place * kManyRows + wave * kResident;
   if (z.shared && w.opens && lane < kResident && row0w + lane < rows) {
     const int row = row0w + lane, token = row / z.group, head = w.head * (int)z.group + row - token * (int)z.group;
-    z.places[(w.s.first + token) * z.head + head] = int2{2 * w.stretch * kManyRows + wave * kResident + lane, w.parts};
+    z.places[(w.s.first + token) * z.head + head] = int2{paged_first_row(w.stretch, w.parts, kManyRows) + wave * kResident + lane, w.parts};
   }
   if (!w.whole && lane < kResident && row0w + lane < rows) z.part_ml[slot0 + lane] = l_tot == 0.f ? float2{-INFINITY, none} : float2{mc, l_tot};
 #pragma unroll

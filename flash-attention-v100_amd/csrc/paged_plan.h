@@ -110,6 +110,9 @@ FMHA_HOST_DEVICE int paged_spread(int w, int stretches) {
 // Where parts of an item that begins in stretch r lie: stretch s has two places, 2 s for the end of an item and 2 s + 1 for the
 // beginning of one.  An item that is all of a stretch and more, begun before, is an end.
 FMHA_HOST_DEVICE int paged_place(int r, int part) { return 2 * (r + part) + (part == 0 ? 1 : 0); }
+// What the table of a row's parts says of an item that begins in stretch r: the row of its place, with slot_rows rows to a place, less
+// slot_rows.  Whole items, of which there may be many more than stretches, have no place.
+FMHA_HOST_DEVICE int paged_first_row(int r, int parts, int slot_rows) { return parts > 1 ? 2 * r * slot_rows : 0; }
 // Whether a row's parts lie among the places, of slot_rows rows each: the first at row `at` + slot_rows, the next ones twice that apart.
 FMHA_HOST_DEVICE bool paged_parts_fit(int at, int parts, int slot_rows) {
   return at >= 0 && parts > 1 && at + 2l * (parts - 1) * slot_rows < 2l * kPagedGroups * slot_rows;
