@@ -348,23 +348,19 @@ struct Walk {
     r.s.n = __builtin_amdgcn_readlane(mine.n, l);
     r.s.keys = __builtin_amdgcn_readlane(mine.keys, l);
     r.s.past = __builtin_amdgcn_readlane(mine.past, l);
-    const int rows = r.s.n * a.group, blocks = B::count(rows);
+    const int rows = r.s.n * a.group, blocks = B::count(rows), rows_of_block = B::rows_of_block(rows);
+    auto scalar = [](int x) __attribute__((always_inline)) { return same(x); };
     if (way != kStretches) {
-      const int each = __builtin_amdgcn_readlane(parts, l), of_head = blocks * each;
-      const int local = at - (__builtin_amdgcn_readlane(upto, l) - of_head * (int)a.kv_head);
+      const int each = __builtin_amdgcn_readlane(parts, l);
+      const int local = at - (__builtin_amdgcn_readlane(upto, l) - blocks * each * (int)a.kv_head);
       int part = 0;
-      if (way == kWhole) {
-        paged_whole_item(local, blocks, a.kv_head, r.block, r.head);
-      } else {
-        r.head = same(paged_divide(local, of_head));
-        r.block = same(paged_divide(local - r.head * of_head, each));
-        part = local - r.head * of_head - r.block * each;
-      }
+      if (way == kWhole) paged_whole_item(local, blocks, a.kv_head, r.block, r.head);
+      else paged_part_item(local, blocks, each, r.block, r.head, part, scalar);
       r.block = same(r.block), r.head = same(r.head);
-      const int tiles = tiles_of(a, r, rows);
-      const float per = (float)tiles * __builtin_amdgcn_rcpf((float)each);  // the same in all parts
-      r.t0 = part == 0 ? 0 : same((int)((float)part * per));
-      r.t1 = part + 1 == each ? tiles : same((int)((float)(part + 1) * per));
+      const int tiles = paged_tiles_of(r.s.keys, r.s.n, a.group, rows_of_block, r.block, a.causal);
+      const float per = (float)tiles * __builtin_amdgcn_rcpf((float)each);
+      r.t0 = same(paged_part_tile(tiles, part, each, per));
+      r.t1 = same(paged_part_tile(tiles, part + 1, each, per));
       r.opens = part == 0;
       r.whole = each == 1;
       r.parts = each;
@@ -373,26 +369,16 @@ struct Walk {
       at = way == kWhole && a.shared ? same(paged_whole(++round, blockIdx.x, items)) : items;
       return true;
     }
-    const PagedLine heads = weights(a, r.s.n, r.s.keys);
-    const long of_head = heads.all(), base = of_lane(line_upto, l) - of_head * a.kv_head;
-    r.head = same(paged_divide(x - base, of_head));
-    const long from = base + r.head * of_head;
-    r.block = blocks == 1 ? 0 : same(paged_block_at(heads, x - from));
-    const long item = from + heads.before(r.block), weight = heads.of(r.block);
-    const int tiles = tiles_of(a, r, rows);
-    r.t0 = same(paged_tile_at(tiles, x - item, weight));
-    r.t1 = same(paged_tile_at(tiles, end - item, weight));
-    r.opens = same((int)(item >= x));
-    r.whole = r.opens && same((int)(item + weight <= end));
-    r.parts = r.whole || !r.opens ? 1 : same(paged_divide(item + weight - 1, length)) - stretch + 1;
-    r.place = paged_place(stretch, r.opens ? 0 : 1) - (r.opens ? 0 : 2);
+    const PagedLine line = weights(a, r.s.n, r.s.keys);
+    PagedShare share;
+    paged_item_at(line, of_lane(line_upto, l) - line.all() * a.kv_head, x, share, scalar);
+    const int tiles = paged_tiles_of(r.s.keys, r.s.n, a.group, rows_of_block, share.block, a.causal);
+    paged_share_of_stretch(tiles, x, end, length, stretch, share, scalar);
+    r.head = share.head, r.block = share.block, r.t0 = share.t0, r.t1 = share.t1;
+    r.opens = share.opens, r.whole = share.whole, r.parts = share.parts, r.place = share.place;
     r.stretch = stretch;
-    x = same(item + weight);
+    x = same(share.item + share.weight);
     return true;
-  }
-  __device__ __forceinline__ static int tiles_of(const PagedArgs& a, const Part& r, int rows) {
-    const int last = min(rows, (r.block + 1) * B::rows_of_block(rows)) - 1;
-    return paged_tiles(paged_visible(r.s.keys, r.s.n, last / a.group, a.causal));
   }
 };
 

@@ -54,6 +54,13 @@ FMHA_HOST_DEVICE int paged_divide(Int n, Int d) {
   return q;
 }
 
+// Tiles of block `block` of a sequence's rows: those that the last of its rows sees.
+template <typename Int>
+FMHA_HOST_DEVICE int paged_tiles_of(int keys, int new_tokens, const Int& group, int rows_of_block, int block, bool causal) {
+  const int rows = new_tokens * group, end = (block + 1) * rows_of_block, last = (rows < end ? rows : end) - 1;
+  return paged_tiles(paged_visible(keys, new_tokens, last / group, causal));
+}
+
 // Length of a stretch: the same for up to kPagedGroups of them, which is as many work groups as the device runs at a time, but
 // not so short that a work group has little else to do than to begin and end.  With 128, 256 and 512 keys at least, us: one token over
 // 1500 keys 10.7, 11.5, 12.0; 64 over 200, 8 key heads, which 128 splits, 16.0, 12.2, 11.6; 200 of those 32.4, 26.9, 26.9.
@@ -87,6 +94,50 @@ FMHA_HOST_DEVICE int paged_tile_at(int tiles, long into, long weight) {
   return at < tiles ? at : tiles;
 }
 
+// Where parts of an item that begins in stretch r lie: stretch s has two places, 2 s for the end of an item and 2 s + 1 for the
+// beginning of one.  An item that is all of a stretch and more, begun before, is an end.
+FMHA_HOST_DEVICE int paged_place(int r, int part) { return 2 * (r + part) + (part == 0 ? 1 : 0); }
+
+// In the functions below `same` returns its argument, which all lanes of a wave have: the kernels put it into a scalar register.
+
+// What a stretch from x to `end` takes of the item at x: its block and key head, tiles t0 .. t1 - 1, whether it begins here and is whole,
+// how many parts it has if it begins here, and the place of this one.  `begin`: where the sequence's first key head lies in the line.
+struct PagedShare {
+  int head, block, t0, t1, parts, place;
+  bool opens, whole;
+  long item, weight;
+};
+template <typename Same>
+FMHA_HOST_DEVICE void paged_item_at(const PagedLine& line, long begin, long x, PagedShare& r, Same same) {
+  const long of_head = line.all();
+  r.head = same(paged_divide(x - begin, of_head));
+  const long from = begin + r.head * of_head;
+  r.block = line.blocks == 1 ? 0 : same(paged_block_at(line, x - from));
+  r.item = from + line.before(r.block), r.weight = line.of(r.block);
+}
+template <typename Same>
+FMHA_HOST_DEVICE void paged_share_of_stretch(int tiles, long x, long end, long length, int stretch, PagedShare& r, Same same) {
+  r.t0 = same(paged_tile_at(tiles, x - r.item, r.weight));
+  r.t1 = same(paged_tile_at(tiles, end - r.item, r.weight));
+  r.opens = same((int)(r.item >= x));
+  r.whole = r.opens && same((int)(r.item + r.weight <= end));
+  r.parts = r.whole || !r.opens ? 1 : same(paged_divide(r.item + r.weight - 1, length)) - stretch + 1;
+  r.place = paged_place(stretch, r.opens ? 0 : 1) - (r.opens ? 0 : 2);
+}
+
+// Part `at` of a sequence's, where each of its items has `each`.
+template <typename Same>
+FMHA_HOST_DEVICE void paged_part_item(int at, int blocks, int each, int& block, int& head, int& part, Same same) {
+  const int of_head = blocks * each;
+  head = same(paged_divide(at, of_head));
+  block = same(paged_divide(at - head * of_head, each));
+  part = at - head * of_head - block * each;
+}
+// First tile of a part, or the end of the last one; per: about tiles / parts, the same for all of them.
+FMHA_HOST_DEVICE int paged_part_tile(int tiles, int part, int parts, float per) {
+  return part == 0 ? 0 : part == parts ? tiles : (int)((float)part * per);
+}
+
 // Item that work group w takes in a round of whole ones: as the persistent kernels for equal lengths, or, if there is one round only,
 // as those of which two share a CU.
 FMHA_HOST_DEVICE int paged_whole(int round, int w, int items) {
@@ -107,9 +158,6 @@ FMHA_HOST_DEVICE int paged_spread(int w, int stretches) {
   return (w >> 3) < run ? (w & 7) * run + (w >> 3) : stretches;
 }
 
-// Where parts of an item that begins in stretch r lie: stretch s has two places, 2 s for the end of an item and 2 s + 1 for the
-// beginning of one.  An item that is all of a stretch and more, begun before, is an end.
-FMHA_HOST_DEVICE int paged_place(int r, int part) { return 2 * (r + part) + (part == 0 ? 1 : 0); }
 // What the table of a row's parts says of an item that begins in stretch r: the row of its place, with slot_rows rows to a place, less
 // slot_rows.  Whole items, of which there may be many more than stretches, have no place.
 FMHA_HOST_DEVICE int paged_first_row(int r, int parts, int slot_rows) { return parts > 1 ? 2 * r * slot_rows : 0; }
