@@ -487,8 +487,8 @@ __device__ __forceinline__ float over_groups_sum(float x) {
 // sums are joined in LDS.
 //
 // Bound by reading the cache, and for short ones by what waits for what: lengths, pages, keys, the sums of the parts.  4 rows a key
-// head, 8 key heads of 128: 131072 keys of one sequence 103 us, 5.2 TB/s of 6.0 that reads alone reach; 8 of about 4096 24.4 us, 3.8 TB/s,
-// of which 4.5 for the join; 32 of 8192 in 8 bits 78 us, 4.0 TB/s, where the copies by themselves take 76 (128 bytes of each KiB at a time).
+// head, 8 key heads of 128: 131072 keys of one sequence 104 us, 5.2 TB/s of 6.0 that reads alone reach; 8 of about 4096 24.8 us, 3.7 TB/s,
+// of which 4.5 for the join; 32 of 8192 in 8 bits 79 us, 4.0 TB/s, where the copies by themselves take 76 (128 bytes of each KiB at a time).
 //
 // 16-bit cache: a unit comes to registers while the one before is worked on, then goes to the tile.
 // 8-bit cache: units are copied to LDS as they are, two at a time, and converted where they become operands.  Keys' scales go into
@@ -926,12 +926,13 @@ __device__ __forceinline__ void few_rows(const PagedArgs& a, const Part& w, char
 // Attention, blocks of 128 rows.  Work group = 4 waves of 32 rows each, one per SIMD, two work groups to a CU; K and V in tiles of 64
 // keys with two slots of LDS each, 16 rows of a tile copied by each wave from one page.  The steps are those of the 128-query
 // forward for equal lengths: softmax(j) with the MFMAs of accumulate(j - 1) and scores(j + 1) between its vector
-// instructions, the running maximum raised only where a tile's probabilities come out too large.  New tokens stand anywhere
+// instructions, the running maximum raised only where a tile's probabilities come out too large: written out here and there, so that a
+// mistake in one is to be looked for in the other.  New tokens stand anywhere
 // against the tiles, so up to two tiles of a wave need a mask; they are done after the main loop.
 //
-// Bound by the MFMAs with what stands between them: 4096 new tokens of 32768, 32 heads of 128, fp16 1808 us, 1.14 PFLOP/s of the
-// 1.24 that a large library product reaches; 2048 of 16384 475 us, 1.08 (bf16 446, 1.16; 8-bit cache 530, 0.97; heads of 64 294, 0.88).
-// With few blocks, by the parts' sums, 64 KiB each, and by the beginnings: 512 of 8192 81 us, 0.82 PFLOP/s, 10 of them for the join.
+// Bound by the MFMAs with what stands between them: 4096 new tokens of 32768, 32 heads of 128, fp16 1845 us, 1.12 PFLOP/s of the
+// 1.24 that a large library product reaches; 2048 of 16384 475 us, 1.09 (bf16 445, 1.16; 8-bit cache 519, 0.99; heads of 64 290, 0.89).
+// With few blocks, by the parts' sums, 64 KiB each, and by the beginnings: 512 of 8192 83 us, 0.80 PFLOP/s, 10 of them for the join.
 // ---------------------------------------------------------------------------
 template <int D, bool Q8>
 struct ManyGeom {
@@ -1995,7 +1996,7 @@ const char* paged_mha_error_string(int code) {
     case FUSED_MHA_ERR_LAUNCH: return "the HIP runtime refused the launch";
     case FUSED_MHA_ERR_BAD_SCALE: return "softmax scale must be finite";
     case FUSED_MHA_ERR_TOO_LARGE: return "the problem is too large";
-    case FUSED_MHA_ERR_BAD_STRIDE: return "strides must be non-negative, with rows on 16-byte boundaries";
+    case FUSED_MHA_ERR_BAD_STRIDE: return "strides must be non-negative and not too large, with rows on 16-byte boundaries";
     case PAGED_MHA_ERR_BAD_TYPE: return "types must be fp16 or bf16, the cache of the same type or e4m3 with scales";
     case PAGED_MHA_ERR_BAD_PAGE_SIZE: return "page size must be a multiple of 16";
     case PAGED_MHA_ERR_BAD_GROUP: return "query heads must be a multiple of key heads";

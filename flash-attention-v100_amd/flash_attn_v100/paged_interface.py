@@ -4,7 +4,7 @@ No counterpart in the reference, whose attention is over queries, keys and value
 The cache is two tensors ``k_cache`` and ``v_cache`` of shape (pages, page_size, kv_heads, head_size), page_size a multiple of
 16, head_size 64 or 128, in fp16 or bf16 as q, k and v are, or in torch.float8_e4m3fn with scales ``k_scale`` and ``v_scale`` of
 shape (pages, page_size, kv_heads) in torch.float8_e8m0fnu.  Strides are free as long as rows of head_size elements are
-contiguous and begin on 16-byte boundaries; pages that hold head by head (a transpose(1, 2) of such a tensor) are read up to a
+contiguous and begin on 16-byte boundaries, slots less than 2 ** 24 and heads less than 2 ** 30 elements apart; pages that hold head by head (a transpose(1, 2) of such a tensor) are read up to a
 tenth faster.
 
 ``page_table`` (batch, columns), int32: position p of sequence b is slot p % page_size of page
@@ -39,8 +39,10 @@ def flash_attn_paged_func(q, k_cache, v_cache, page_table, cache_seqlens, softma
     q has a multiple of the cache's heads: query head h attends to head h // (heads // kv_heads).  causal: a token sees keys up to
     its own position, otherwise all of its sequence.  Rows that see no key are zero.  Keys that a token does not see do not matter to
     it, whatever they and their values hold.  softmax_scale: head_size ** -0.5 if None.
-    max_seqlen: no sequence has more new tokens (with cu_seqlens; helps to pick the kernel, is not needed for the result).
-    out: dense tensor of q's shape to write to; rows of tokens that belong to no sequence stay as they are there, and are zero
+    max_seqlen: no sequence has more new tokens (with cu_seqlens).  Not needed for the result, but without it all tokens could be one
+    sequence's: 64 single tokens over about 4096 keys each, 32 heads of 128, then take 179 us instead of 163, 16 over 2000 35 instead of
+    27, out of 8 bits 31 instead of 21, with a workspace of 65 MiB instead of 8; a batch with chunks takes as long either way.
+    out: dense tensor of q's shape on a 16-byte boundary to write to, which shares no memory with the others; rows of tokens that belong to no sequence stay as they are there, and are zero
     in a tensor made here.  Returns it."""
     return _attention(q, k_cache, v_cache, page_table, cache_seqlens, softmax_scale, causal, cu_seqlens, max_seqlen,
                       k_scale, v_scale, out)

@@ -87,7 +87,8 @@ int paged_mha_read(const paged_mha_cache *cache, const paged_mha_batch *batch, i
  * position.  head is a multiple of kv_head; query head h has key head h / (head / kv_head).  A row without keys is zero,
  * one all of whose scores are -inf NaN.
  * Keys that a row does not see do not matter to it, whatever they and their values hold.
- * o is dense.  max_new: no sequence has more new tokens (0: not known); which kernel is taken goes by it, not the result.
+ * o is dense.  max_new: no sequence has more new tokens (0: not known); which kernel and how much workspace is taken
+ * goes by it, not the result.
  * zero_rest: rows of o that belong to no sequence (tokens in front of cu_seqlens[0], and from cu_seqlens[batch] on) are zeroed
  * instead of left.
  * The workspace holds parts of long sequences that several work groups share; its contents do not matter before or after.
